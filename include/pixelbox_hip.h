@@ -392,6 +392,58 @@ int pb_phash_batch_images(pb_phasher *p, const uint8_t *const *rgb, const uint32
 int pb_phash_small_image(pb_phasher *p, const uint8_t *rgb, uint32_t width, uint32_t height, uint8_t *out_rgb, uint32_t *out_w, uint32_t *out_h);
 
 /* ======================================================================================
+ *  linear layers on device buffers: what the network's own last layer is (Linear(1280, D) + tanh, resources/train.py:30-46), for
+ *  layers of the caller's -- in 8 bits, or one set of weights per GROUP of rows (hash heads of several collections on one backbone,
+ *  experts).
+ *
+ *  All pointers are DEVICE memory of `device`; `stream` is the hipStream_t the work is queued on (NULL: the device's null stream).
+ *  A call checks its arguments, queues one kernel and returns: outputs are complete for later work on that stream, or once the
+ *  caller has waited for it.  Nothing is allocated and no state outlives a call, so calls may run from any threads, on any streams,
+ *  and inside a graph capture.  m = 0 (and n = 0) is a call that does nothing.
+ *  ld* is the distance between rows in ELEMENTS; any value >= the row length, any alignment of a row to its type.  16-byte aligned
+ *  rows run fastest.
+ * ====================================================================================== */
+#define PB_TYPE_F32 0
+#define PB_TYPE_BF16 1
+#define PB_TYPE_F16 2
+#define PB_TYPE_I8 3
+#define PB_ACT_NONE 0
+#define PB_ACT_SILU 1 /* v / (1 + e^-v) */
+#define PB_ACT_TANH 2
+#define PB_MAX_GROUPS 1024u
+#define PB_LINEAR_I8_MAX_K 131071u /* (-128)^2 * k stays below 2^31 */
+
+/* Rows of floats (f32, bf16, f16) -> codes in [-127, 127] and one scale per row: scale = max(max |x| / 127, 2^-126) rounded to f32,
+ * code = x / scale to the nearest whole number, halves to the even one, decided exactly.  A row of zeros (or of no values) has
+ * codes 0; a row that holds an infinity or a NaN has codes 0 and scale NaN, so that every product of it is NaN.  With the
+ * rows of a weight matrix [n][k] it gives the codes and channel scales of pb_linear_i8.  x: [m][ldx], codes: int8 [m][ldc],
+ * scale: f32[m]. */
+int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale);
+
+/* y[r][c] = act( (sum_k x[r][k] w[c][k]) * x_scale[r] * w_scale[c] + bias[c] ): the sum in 32-bit integers (exact), the rest in
+ * f32, one rounding to y's type (f32, bf16, f16).  x: int8 [m][ldx], w: int8 [n][ldw], bias: f32[n] or NULL, y: [m][ldy].
+ * The result does not depend on m or on the kernel chosen. */
+int pb_linear_i8(int device, void *stream, const void *x, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw, const float *w_scale,
+                 const float *bias, int act, void *y, int y_type, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k);
+
+/* The group of each row -> the rows in the order of their groups.  group: int[m]; order: int[m], the rows of group 0 in ascending
+ * order, then those of group 1, ...; offsets: int[groups + 1], group g's rows are order[offsets[g] .. offsets[g + 1]).  Rows whose
+ * group is negative or >= groups have none: they are listed (ascending) behind offsets[groups]. */
+int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32_t groups, int *offsets, int *order);
+
+/* For every group g and position r in [offsets[g], offsets[g + 1]), with xr = x_rows ? x_rows[r] : r and yr likewise:
+ *   y[yr] = act( (x[xr] . w[g]^T) (* x_scale[xr] * w_scale[g]) + bias[g] )
+ * type: f32, bf16, f16 (products summed in f32) or i8 (as pb_linear_i8; x_scale f32[x_total] and w_scale f32[groups][n], ignored
+ * for the others).  w: [groups][n][ldw], bias: f32[groups][n] or NULL.  With x_rows = y_rows = pb_group_rows' order, y is in the
+ * order of x; with only x_rows the groups' results lie packed, as the input of a next layer that has only y_rows.  offsets
+ * (int[groups + 1]) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,
+ * a row number outside x ([0, x_total)) or y ([0, y_total)) is skipped.  A row of x may be listed any number of times, a row of y
+ * once (twice: either result stands).  Rows of y that are not listed are left as they are.  y must not overlap x or w. */
+int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
+                      const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
+                      void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k);
+
+/* ======================================================================================
  *  utilities
  * ====================================================================================== */
 /* splitmix64 byte stream on the device: d_out[0..nbytes) = bytes [byte_offset, ..) of stream `seed`

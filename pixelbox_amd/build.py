@@ -22,8 +22,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libpixelbox_hip.so")
 STAMP = LIB + ".stamp"
-SOURCES = ["pb_scan.hip", "pb_embed.hip", "pb_gemm_p3.hip", "pb_sharded.hip", "pb_phash.hip"]
-HEADERS = ["pb_common.h", "pb_scan_kernels.h", "pb_embed_common.h", "pb_embed_kernels.h", "pb_gemm_p3.h", "pb_p3_common.h", "pb_gemm_p3_launch.h", "pb_front_band.h", "pb_block_small.h", "pb_phash_kernels.h", "pb_merge_kernels.h",
+SOURCES = ["pb_scan.hip", "pb_embed.hip", "pb_gemm_p3.hip", "pb_sharded.hip", "pb_phash.hip", "pb_linear.hip"]
+HEADERS = ["pb_common.h", "pb_scan_kernels.h", "pb_embed_common.h", "pb_embed_kernels.h", "pb_gemm_p3.h", "pb_p3_common.h", "pb_gemm_p3_launch.h", "pb_front_band.h", "pb_block_small.h", "pb_phash_kernels.h", "pb_merge_kernels.h", "pb_linear_kernels.h",
            os.path.join("..", "..", "include", "pixelbox_hip.h")]
 # no packed f32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this chip now and then (the
 # host pass of hipcc warns that it does not know the feature: harmless)

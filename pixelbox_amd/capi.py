@@ -33,6 +33,10 @@ PB_ERR_RANGE = -7  # embed: an activation left the domain of the fixed-point squ
 PB_OPT_EMBED_ASYNC = 4   # pb_embed_set_option: 1 = pb_embed_batch_device returns with the forward pass queued (default 0: waits)
 PB_OPT_SCAN_LAUNCH = 8  # 0: one launch per query; 1: queries side by side in one grid; 2 (default): one launch, queries one after the other
 PB_METRIC_COSINE, PB_METRIC_BYTE, PB_METRIC_HAMMING = 0, 1, 2
+PB_TYPE_F32, PB_TYPE_BF16, PB_TYPE_F16, PB_TYPE_I8 = 0, 1, 2, 3
+PB_ACT_NONE, PB_ACT_SILU, PB_ACT_TANH = 0, 1, 2
+PB_MAX_GROUPS = 1024
+PB_LINEAR_I8_MAX_K = 131071
 
 # every symbol include/pixelbox_hip.h declares (tests/test_abi.py checks the header against this list
 # and the built library against both)
@@ -47,6 +51,7 @@ SYMBOLS = [
     "pb_mlhash_image", "pb_embed_batch_images", "pb_embed_batch_images_device", "pb_embed_stage_acquire", "pb_embed_stage_release", "pb_embed_stage_close",
     "pb_embed_stage_commit", "pb_embed_stage_abort", "pb_resize_to_fill",
     "pb_embed_set_option", "pb_pinned_alloc", "pb_pinned_free", "pb_embed_tune_ms", "pb_embed_get_tuning", "pb_embed_set_tuning", "pb_fill_synthetic", "pb_fill_synthetic_images", "pb_fill_synthetic_scenes",
+    "pb_quantize_rows", "pb_linear_i8", "pb_group_rows", "pb_linear_grouped",
     "pb_phash_create", "pb_phash_destroy", "pb_phash_image", "pb_phash_batch_images", "pb_phash_small_image",
 ]
 
@@ -149,6 +154,11 @@ def lib():
         L.pb_fill_synthetic.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, vp]
         L.pb_fill_synthetic_images.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, vp]
         L.pb_fill_synthetic_scenes.argtypes = [C.c_int, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, vp]
+        u32, u64 = C.c_uint32, C.c_uint64
+        L.pb_quantize_rows.argtypes = [C.c_int, vp, vp, C.c_int, u64, u32, u64, vp, u64, vp]
+        L.pb_linear_i8.argtypes = [C.c_int, vp, vp, u64, vp, vp, u64, vp, vp, C.c_int, vp, C.c_int, u64, u64, u32, u32]
+        L.pb_group_rows.argtypes = [C.c_int, vp, vp, u64, u32, vp, vp]
+        L.pb_linear_grouped.argtypes = [C.c_int, vp, C.c_int, vp, u64, u64, vp, vp, u64, vp, vp, vp, u32, vp, vp, C.c_int, vp, C.c_int, u64, u64, u64, u32, u32]
         _lib = L
     return _lib
 

@@ -1,0 +1,206 @@
+// pb_linear.hip -- C entry points of the linear layers on device buffers (kernels: pb_linear_kernels.h).
+//
+// Each call checks its arguments on the host, queues ONE kernel on the caller's stream and returns.  Nothing is allocated, no
+// state outlives a call: calls on any number of streams and from any number of threads are independent, and a captured graph
+// holds nothing that another one shares.
+#include <algorithm>
+#include <climits>
+
+#include "pb_common.h"
+#include "pb_linear_kernels.h"
+
+using namespace pbl;
+
+namespace {
+
+// the caller's device for the duration of a call; the device is left alone where it is the current one already
+struct Device {
+    int prev = -1;
+    bool ok = true;
+    explicit Device(int dev) {
+        int cur = -1;
+        ok = hipGetDevice(&cur) == hipSuccess;
+        if (ok && cur != dev) {
+            ok = hipSetDevice(dev) == hipSuccess;
+            prev = cur;
+        }
+    }
+    ~Device() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+// bytes from the first row to the end of the last one
+uint64_t extent(uint64_t rows, uint64_t ld, uint64_t n, int size) { return rows && n ? ((rows - 1) * ld + n) * size : 0; }
+bool bad_type(int t) { return t != PB_TYPE_F32 && t != PB_TYPE_BF16 && t != PB_TYPE_F16; }
+bool misaligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(size - 1)) != 0; }
+
+constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 stays far inside 64 bits
+
+template <int T, int BM, int BN, int WM, int WN>
+void launch_tile(const LinearArgs &a, bool dma, long m_tiles, hipStream_t s) {
+    const dim3 grid((unsigned)((m_tiles * a.n_tiles + 7) / 8 * 8)), block(64 * (BM / WM) * (BN / WN));
+    if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WM, WN, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WM, WN, false>), grid, block, 0, s, a);
+}
+template <int T, int MT, int NT, int NW>
+void launch_few(const LinearArgs &a, bool aligned, long m_tiles, hipStream_t s) {
+    const dim3 grid((unsigned)((m_tiles * a.n_tiles + 7) / 8 * 8)), block(64 * NW);
+    if (aligned) hipLaunchKernelGGL((k_linear_few<T, MT, NT, NW, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((k_linear_few<T, MT, NT, NW, false>), grid, block, 0, s, a);
+}
+
+template <int T>
+int launch(LinearArgs a, hipStream_t s) {
+    const bool aligned = !misaligned(a.x, 16) && !misaligned(a.w, 16) && a.ldx % 16 == 0 && a.ldw % 16 == 0;
+    // tiles of BM rows that the groups can have: every group but the largest may end inside one
+    auto m_tiles = [&](long bm) { return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm; };
+    auto n_tiles = [&](long bn) { return (a.n + bn - 1) / bn; };
+    const long mt64 = m_tiles(64) , mt16 = m_tiles(16);
+    const long tiles64 = mt64 * n_tiles(64);
+    if (a.m / a.groups >= 32 && tiles64 >= 192) {
+        a.n_tiles = (int)n_tiles(64);
+        PB_CHECK(mt64 * a.n_tiles < INT_MAX - 8, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
+        launch_tile<T, 64, 64, 32, 32>(a, aligned, mt64, s);
+    } else {
+        a.n_tiles = (int)n_tiles(16);
+        PB_CHECK(mt16 * a.n_tiles < INT_MAX - 8, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
+        launch_few<T, 1, 1, 8>(a, aligned, mt16, s);
+    }
+    PB_HIP(hipGetLastError());
+    return PB_OK;
+}
+
+// what pb_linear_i8 and pb_linear_grouped have in common
+int linear(const char *who, int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w,
+           uint64_t ldw, const float *w_scale, const float *bias, const int32_t *offsets, uint32_t groups, const int32_t *x_rows,
+           const int32_t *y_rows, int act, void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k) {
+    const bool i8 = type == PB_TYPE_I8;
+    PB_CHECK(i8 || !bad_type(type), PB_ERR_INVALID, "%s: unknown type %d", who, type);
+    PB_CHECK(!bad_type(y_type), PB_ERR_INVALID, "%s: unknown output type %d (f32, bf16, f16)", who, y_type);
+    PB_CHECK(act >= PB_ACT_NONE && act <= PB_ACT_TANH, PB_ERR_INVALID, "%s: unknown activation %d", who, act);
+    PB_CHECK(m <= INT_MAX && x_total <= INT_MAX && y_total <= INT_MAX, PB_ERR_INVALID, "%s: more than 2^31 - 1 rows", who);
+    PB_CHECK(n <= (uint32_t)INT_MAX / 2 && k <= (uint32_t)INT_MAX / 4, PB_ERR_INVALID, "%s: n = %u, k = %u is out of range", who, n, k);
+    PB_CHECK(!i8 || k <= PB_LINEAR_I8_MAX_K, PB_ERR_INVALID, "%s: k = %u would overflow 32-bit sums (at most %u)", who, k, PB_LINEAR_I8_MAX_K);
+    PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
+    PB_CHECK(ldx >= k && ldw >= k && ldy >= n && ldx <= MAX_LD && ldw <= MAX_LD && ldy <= MAX_LD, PB_ERR_INVALID,
+             "%s: rows of %u inputs and %u outputs do not fit their strides", who, k, n);
+    if (m == 0 || n == 0) return PB_OK;
+    const int size = type_bytes(type), y_size = type_bytes(y_type);
+    PB_CHECK(y && (k == 0 || (x && w)), PB_ERR_INVALID, "%s: null buffer", who);
+    PB_CHECK(!i8 || (x_scale && w_scale), PB_ERR_INVALID, "%s: 8-bit operands need x_scale and w_scale", who);
+    PB_CHECK(x_total > 0 && y_total > 0, PB_ERR_INVALID, "%s: no rows to read or to write", who);
+    PB_CHECK(x_rows || m <= x_total, PB_ERR_INVALID, "%s: m = %llu rows of an x of %llu", who, (unsigned long long)m, (unsigned long long)x_total);
+    PB_CHECK(y_rows || m <= y_total, PB_ERR_INVALID, "%s: m = %llu rows of a y of %llu", who, (unsigned long long)m, (unsigned long long)y_total);
+    PB_CHECK(!misaligned(x, size) && !misaligned(w, size) && !misaligned(y, y_size), PB_ERR_INVALID, "%s: a buffer is not aligned to its type", who);
+    PB_CHECK(!misaligned(x_scale, 4) && !misaligned(w_scale, 4) && !misaligned(bias, 4) && !misaligned(offsets, 4) && !misaligned(x_rows, 4) &&
+                 !misaligned(y_rows, 4),
+             PB_ERR_INVALID, "%s: a scale, bias or index array is not aligned to 4 bytes", who);
+    const uint64_t y_bytes = extent(y_total, ldy, n, y_size);
+    PB_CHECK(!overlap(y, y_bytes, x, extent(x_total, ldx, k, size)) && !overlap(y, y_bytes, w, extent((uint64_t)groups * n, ldw, k, size)), PB_ERR_INVALID,
+             "%s: y overlaps an operand", who);
+    Device dev(device);
+    PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
+    LinearArgs a;
+    a.x = static_cast<const uint8_t *>(x);
+    a.w = static_cast<const uint8_t *>(w);
+    a.x_scale = x_scale;
+    a.w_scale = w_scale;
+    a.bias = bias;
+    a.offsets = offsets;
+    a.x_rows = x_rows;
+    a.y_rows = y_rows;
+    a.y = static_cast<uint8_t *>(y);
+    a.ldx = (long)ldx * size;
+    a.ldw = (long)ldw * size;
+    a.ldy = (long)ldy * y_size;
+    a.kb = (long)k * size;
+    a.m = (int)m;
+    a.n = (int)n;
+    a.groups = (int)groups;
+    a.n_tiles = 0;
+    a.x_total = (int)x_total;
+    a.y_total = (int)y_total;
+    a.act = act;
+    a.y_type = y_type;
+    a.y_vec = !misaligned(y, 16) && a.ldy % 16 == 0;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (type) {
+        case PB_TYPE_F32: return launch<F32>(a, s);
+        case PB_TYPE_BF16: return launch<BF16>(a, s);
+        case PB_TYPE_F16: return launch<F16>(a, s);
+        default: return launch<I8>(a, s);
+    }
+}
+
+template <int T, bool VEC>
+void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, int8_t *codes, uint64_t ldc, float *scale, hipStream_t s) {
+    const uint8_t *px = static_cast<const uint8_t *>(x);
+    hipLaunchKernelGGL((k_quantize_rows<T, 256, 4, VEC>), dim3((unsigned)m), dim3(256), 0, s, px, (long)m, (int)k, (long)ldx * type_bytes(T), codes, (long)ldc,
+                       scale);
+}
+
+}  // namespace
+
+extern "C" {
+
+int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale) {
+    const char *who = "pb_quantize_rows";
+    PB_CHECK(!bad_type(x_type), PB_ERR_INVALID, "%s: unknown type %d (f32, bf16, f16)", who, x_type);
+    PB_CHECK(m <= INT_MAX && k <= (uint32_t)INT_MAX / 4, PB_ERR_INVALID, "%s: m = %llu, k = %u is out of range", who, (unsigned long long)m, k);
+    PB_CHECK(ldx >= k && ldc >= k && ldx <= MAX_LD && ldc <= MAX_LD, PB_ERR_INVALID, "%s: rows of %u values do not fit their strides", who, k);
+    if (m == 0) return PB_OK;
+    const int size = type_bytes(x_type);
+    PB_CHECK(scale && (k == 0 || (x && codes)), PB_ERR_INVALID, "%s: null buffer", who);
+    PB_CHECK(!misaligned(x, size) && !misaligned(scale, 4), PB_ERR_INVALID, "%s: a buffer is not aligned to its type", who);
+    const uint64_t xb = extent(m, ldx, k, size), cb = extent(m, ldc, k, 1);
+    PB_CHECK(!overlap(codes, cb, x, xb) && !overlap(scale, m * 4, x, xb) && !overlap(scale, m * 4, codes, cb), PB_ERR_INVALID, "%s: buffers overlap", who);
+    Device dev(device);
+    PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int v = x_type == PB_TYPE_F32 ? 4 : 8;
+    const bool vec = !misaligned(x, 16) && ldx * size % 16 == 0 && !misaligned(codes, v) && ldc % v == 0;
+    switch (x_type) {
+        case PB_TYPE_F32: vec ? launch_quantize<F32, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<F32, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
+        case PB_TYPE_BF16: vec ? launch_quantize<BF16, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<BF16, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
+        default: vec ? launch_quantize<F16, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<F16, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
+    }
+    PB_HIP(hipGetLastError());
+    return PB_OK;
+}
+
+int pb_linear_i8(int device, void *stream, const void *x, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw, const float *w_scale,
+                 const float *bias, int act, void *y, int y_type, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k) {
+    return linear("pb_linear_i8", device, stream, PB_TYPE_I8, x, m, ldx, x_scale, w, ldw, w_scale, bias, nullptr, 1, nullptr, nullptr, act, y, y_type, m, ldy,
+                  m, n, k);
+}
+
+int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32_t groups, int *offsets, int *order) {
+    const char *who = "pb_group_rows";
+    PB_CHECK(m <= INT_MAX, PB_ERR_INVALID, "%s: more than 2^31 - 1 rows", who);
+    PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
+    PB_CHECK(offsets && (m == 0 || (group && order)), PB_ERR_INVALID, "%s: null buffer", who);
+    PB_CHECK(!misaligned(group, 4) && !misaligned(offsets, 4) && !misaligned(order, 4), PB_ERR_INVALID, "%s: a buffer is not aligned to 4 bytes", who);
+    PB_CHECK(!overlap(group, m * 4, order, m * 4) && !overlap(group, m * 4, offsets, (groups + 1ull) * 4) && !overlap(order, m * 4, offsets, (groups + 1ull) * 4),
+             PB_ERR_INVALID, "%s: buffers overlap", who);
+    Device dev(device);
+    PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
+    hipLaunchKernelGGL(k_group_rows, dim3(groups + 1), dim3(64 * GR_WAVES), 0, static_cast<hipStream_t>(stream), group, (int)m, (int)groups,
+                       (int)!misaligned(group, 16), offsets, order);
+    PB_HIP(hipGetLastError());
+    return PB_OK;
+}
+
+int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
+                      const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
+                      void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k) {
+    PB_CHECK(offsets || m == 0, PB_ERR_INVALID, "pb_linear_grouped: null offsets");
+    return linear("pb_linear_grouped", device, stream, type, x, x_total, ldx, x_scale, w, ldw, w_scale, bias, offsets, groups, x_rows, y_rows, act, y, y_type,
+                  y_total, ldy, m, n, k);
+}
+
+}  // extern "C"

@@ -1,0 +1,212 @@
+"""Linear layers on torch tensors: 8-bit products with a scale per row and channel, and products grouped by expert.
+
+The tensor-facing form of pb_quantize_rows, pb_linear_i8, pb_group_rows and pb_linear_grouped (include/pixelbox_hip.h): shapes, types,
+strides and devices are checked here, the work is queued on the tensors' device on torch's current stream, and nothing waits for it.
+
+    w_codes, w_scale = quantize_rows(weight)                     # once: weight [n, k] -> codes and a scale per channel
+    codes, scale = quantize_rows(features)                       # per batch
+    y = linear_i8(codes, scale, w_codes, w_scale, bias, act="tanh")
+
+    offsets, order = group_rows(head_of_image, heads)            # images of a batch -> rows in the order of their heads
+    y = linear_grouped(features, weights, offsets, rows=order, bias=bias, act="tanh")   # weights [heads, n, k]
+
+Rows may have any stride >= their length (a slice of a wider tensor), the last axis is contiguous.  Products have no gradient: an
+operand that requires one is refused.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import capi
+
+_TYPES = {torch.float32: capi.PB_TYPE_F32, torch.bfloat16: capi.PB_TYPE_BF16, torch.float16: capi.PB_TYPE_F16, torch.int8: capi.PB_TYPE_I8}
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+_ACTS = {"none": capi.PB_ACT_NONE, "silu": capi.PB_ACT_SILU, "tanh": capi.PB_ACT_TANH}
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _device(t: torch.Tensor, name: str) -> torch.device:
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} is on {t.device}: the operators run on a GPU")
+    return t.device
+
+
+def _check(t: torch.Tensor, name: str, shape: tuple, dtypes, device: torch.device) -> None:
+    """dtype, device, shape (None: any length) and a contiguous last axis; rows do not overlap one another"""
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+    if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
+        raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {shape}")
+    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the last axis is not contiguous")
+
+
+def _ld(t: torch.Tensor, name: str) -> int:
+    """distance between the rows of a 2-d tensor"""
+    n = t.shape[1]
+    if t.shape[0] <= 1:
+        return n
+    ld = t.stride(0)
+    if ld < n:
+        raise ValueError(f"{name}: rows overlap (a stride of {ld} for {n} values)")
+    return ld
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("these products have no gradient: an operand requires one (detach it, or call under torch.no_grad())")
+
+
+def _act(act: str) -> int:
+    if act not in _ACTS:
+        raise ValueError(f"act is {act!r}, not one of {', '.join(_ACTS)}")
+    return _ACTS[act]
+
+
+def _ptr(t) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def _call(rc: int) -> None:
+    if rc != capi.PB_OK:
+        capi._check(rc)
+
+
+def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """x [m, k] (f32, bf16, f16) -> (codes int8 [m, k], scale f32 [m]): scale = max(max |x| / 127, 2^-126) of each row, codes rounded to the
+    nearest, halves to even.  A row with an infinity or a NaN has scale NaN and codes 0."""
+    dev = _device(x, "x")
+    _check(x, "x", (None, None), _FLOATS, dev)
+    _no_grad(x)
+    m, k = x.shape
+    if codes is None:
+        codes = torch.empty((m, k), dtype=torch.int8, device=dev)
+    else:
+        _check(codes, "codes", (m, k), (torch.int8,), dev)
+    if scale is None:
+        scale = torch.empty((m,), dtype=torch.float32, device=dev)
+    else:
+        _check(scale, "scale", (m,), (torch.float32,), dev)
+    ldx, ldc = _ld(x, "x"), _ld(codes, "codes")
+    _call(capi.lib().pb_quantize_rows(dev.index, _stream(dev), x.data_ptr(), _TYPES[x.dtype], m, k, ldx, codes.data_ptr(), ldc, scale.data_ptr()))
+    return codes, scale
+
+
+def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None, act: str = "none",
+              dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
+    """act((x w^T) * x_scale * w_scale + bias): x int8 [m, k], w int8 [n, k], x_scale f32 [m], w_scale f32 [n], bias f32 [n].  The result has
+    `dtype`, or out's."""
+    dev = _device(x, "x")
+    code = _act(act)
+    _check(x, "x", (None, None), (torch.int8,), dev)
+    m, k = x.shape
+    _check(w, "w", (None, k), (torch.int8,), dev)
+    n = w.shape[0]
+    _check(x_scale, "x_scale", (m,), (torch.float32,), dev)
+    _check(w_scale, "w_scale", (n,), (torch.float32,), dev)
+    if bias is not None:
+        _check(bias, "bias", (n,), (torch.float32,), dev)
+    _no_grad(x_scale, w_scale, bias)
+    if out is None:
+        if dtype not in _FLOATS:
+            raise TypeError(f"dtype is {dtype}, not one of {', '.join(str(d) for d in _FLOATS)}")
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+    else:
+        _check(out, "out", (m, n), _FLOATS, dev)
+    ldx, ldw, ldy = _ld(x, "x"), _ld(w, "w"), _ld(out, "out")
+    _call(capi.lib().pb_linear_i8(dev.index, _stream(dev), x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), code,
+                                  out.data_ptr(), _TYPES[out.dtype], ldy, m, n, k))
+    return out
+
+
+def group_rows(group: torch.Tensor, groups: int, offsets: torch.Tensor | None = None, order: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """group int32 [m] -> (offsets int32 [groups + 1], order int32 [m]): group g's rows are order[offsets[g] : offsets[g + 1]], ascending.  Rows with a
+    group outside [0, groups) come last, behind offsets[groups]."""
+    dev = _device(group, "group")
+    _check(group, "group", (None,), (torch.int32,), dev)
+    m = group.shape[0]
+    if not 1 <= groups <= capi.PB_MAX_GROUPS:
+        raise ValueError(f"groups is {groups}, not 1 .. {capi.PB_MAX_GROUPS}")
+    if offsets is None:
+        offsets = torch.empty((groups + 1,), dtype=torch.int32, device=dev)
+    else:
+        _check(offsets, "offsets", (groups + 1,), (torch.int32,), dev)
+    if order is None:
+        order = torch.empty((m,), dtype=torch.int32, device=dev)
+    else:
+        _check(order, "order", (m,), (torch.int32,), dev)
+    _call(capi.lib().pb_group_rows(dev.index, _stream(dev), group.data_ptr(), m, groups, offsets.data_ptr(), order.data_ptr()))
+    return offsets, order
+
+
+def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows: torch.Tensor | None = None, x_rows: torch.Tensor | None = None,
+                   y_rows: torch.Tensor | None = None, x_scale: torch.Tensor | None = None, w_scale: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, act: str = "none", dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[yr(r)] = act(x[xr(r)] w[g]^T (* x_scale[xr(r)] * w_scale[g]) + bias[g]) for every group g and r in [offsets[g], offsets[g + 1]).
+
+    x [rows of x, k] (f32, bf16, f16; int8 with x_scale [rows of x] and w_scale [groups, n]), w [groups, n, k], bias f32 [groups, n], offsets int32
+    [groups + 1].  x_rows and y_rows (int32 [m], `rows` for both) name the row of x that is read and the row of out that is written at each place r;
+    without them it is r itself.  Rows of out that no place names are left as they are: zero where out is made here (m rows, or as many as x has
+    where y_rows is given)."""
+    dev = _device(x, "x")
+    code = _act(act)
+    _check(x, "x", (None, None), _FLOATS + (torch.int8,), dev)
+    x_total, k = x.shape
+    if w.dim() != 3:
+        raise ValueError(f"w has the shape {tuple(w.shape)}, not (groups, n, k)")
+    groups, n, _ = w.shape
+    _check(w, "w", (None, None, k), (x.dtype,), dev)
+    if not 1 <= groups <= capi.PB_MAX_GROUPS:
+        raise ValueError(f"w has {groups} groups, not 1 .. {capi.PB_MAX_GROUPS}")
+    ldw = w.stride(1) if n > 1 else k
+    if ldw < k or (groups > 1 and n > 0 and w.stride(0) != n * ldw):
+        raise ValueError("w: the groups' weights do not follow one another row by row")
+    _check(offsets, "offsets", (groups + 1,), (torch.int32,), dev)
+    if rows is not None:
+        if x_rows is not None or y_rows is not None:
+            raise ValueError("rows stands for x_rows and y_rows: give one or the other")
+        x_rows = y_rows = rows
+    m = x_total
+    for t, name in ((x_rows, "x_rows"), (y_rows, "y_rows")):
+        if t is not None:
+            _check(t, name, (None,), (torch.int32,), dev)
+            m = t.shape[0]
+    if x_rows is not None and y_rows is not None and x_rows.shape[0] != y_rows.shape[0]:
+        raise ValueError(f"x_rows and y_rows differ in length: {x_rows.shape[0]}, {y_rows.shape[0]}")
+    if x_rows is None and m > x_total:
+        raise ValueError(f"y_rows lists {m} rows, x has {x_total}")
+    i8 = x.dtype == torch.int8
+    if i8:
+        if x_scale is None or w_scale is None:
+            raise ValueError("8-bit operands need x_scale and w_scale")
+        _check(x_scale, "x_scale", (x_total,), (torch.float32,), dev)
+        _check(w_scale, "w_scale", (groups, n), (torch.float32,), dev)
+    elif x_scale is not None or w_scale is not None:
+        raise ValueError("scales are for 8-bit operands")
+    if bias is not None:
+        _check(bias, "bias", (groups, n), (torch.float32,), dev)
+    for t, name in ((w_scale, "w_scale"), (bias, "bias")):
+        if t is not None and groups > 1 and n > 0 and t.stride(0) != n:
+            raise ValueError(f"{name}: the groups' rows do not follow one another")
+    _no_grad(x, w, x_scale, w_scale, bias)
+    if out is None:
+        dtype = dtype or (torch.float32 if i8 else x.dtype)
+        if dtype not in _FLOATS:
+            raise TypeError(f"dtype is {dtype}, not one of {', '.join(str(d) for d in _FLOATS)}")
+        out = torch.zeros((m if y_rows is None else max(m, x_total), n), dtype=dtype, device=dev)
+    else:
+        _check(out, "out", (None, n), _FLOATS, dev)
+        if y_rows is None and out.shape[0] < m:
+            raise ValueError(f"out has {out.shape[0]} rows, {m} may be written")
+    if m == 0 or n == 0 or (out.shape[0] == 0 and y_rows is not None) or x_total == 0:
+        return out
+    ldx, ldy = _ld(x, "x"), _ld(out, "out")
+    _call(capi.lib().pb_linear_grouped(dev.index, _stream(dev), _TYPES[x.dtype], x.data_ptr(), x_total, ldx, _ptr(x_scale), w.data_ptr(), ldw,
+                                       _ptr(w_scale), _ptr(bias), offsets.data_ptr(), groups, _ptr(x_rows), _ptr(y_rows), code, out.data_ptr(),
+                                       _TYPES[out.dtype], out.shape[0], ldy, m, n, k))
+    return out
