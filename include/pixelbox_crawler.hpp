@@ -120,10 +120,12 @@ class Crawler {
         for (size_t m = 0; m < models_.size(); ++m) threads_.emplace_back([this, m] { embed_thread(m); });
     }
 
-    // the Receiver<IndexedImage>: blocks for the next image; false once every file has been processed
+    // the Receiver<IndexedImage>: blocks for the next image; false once every file has been processed, or after a cancel or a failure.
+    // In either case every embed thread has left by then: the embedders are the caller's again (a batch that a thread had closed when
+    // cancel() came is committed or discarded, not still between the two).
     bool recv(IndexedImage &out) {
         std::unique_lock<std::mutex> lk(mu_);
-        cv_out_.wait(lk, [&] { return !out_.empty() || out_closed_ || cancelled_; });
+        cv_out_.wait(lk, [&] { return !out_.empty() || out_closed_; });
         if (out_.empty()) return false;
         out = std::move(out_.front());
         out_.pop_front();
@@ -280,6 +282,10 @@ class Crawler {
                     for (;;) {
                         uint8_t *px = nullptr;
                         if (acquired) return nullptr;  // one image per file: a decoder that asks twice gets no second room
+                        {
+                            std::lock_guard<std::mutex> lk(mu_);
+                            if (cancelled_) return nullptr;  // no new batch behind the one that the cancel discarded
+                        }
                         const int rc = pb_embed_stage_acquire(models_[m]->raw(), w, h, &px, &ticket);
                         if (rc == PB_OK) {
                             acquired = true;
@@ -447,7 +453,7 @@ class Crawler {
             cv_space_.notify_all();
         }
         std::lock_guard<std::mutex> lk(mu_);
-        if (--embedders_left_ == 0 || cancelled_) {
+        if (--embedders_left_ == 0) {
             out_closed_ = true;
             cv_out_.notify_all();
         }
