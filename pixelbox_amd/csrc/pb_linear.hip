@@ -41,38 +41,72 @@ bool misaligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(si
 
 constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 stays far inside 64 bits
 
-template <int T, int BM, int BN, int WM, int WN>
-void launch_tile(const LinearArgs &a, bool dma, long m_tiles, hipStream_t s) {
-    const dim3 grid((unsigned)((m_tiles * a.n_tiles + 7) / 8 * 8)), block(64 * (BM / WM) * (BN / WN));
-    if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WM, WN, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WM, WN, false>), grid, block, 0, s, a);
+// The forms of a product.  What a launch costs goes, to within a tenth or two, as 3 us + the number of rounds of workgroups it takes
+// times a form's own time per round and summed byte, whatever the type's size -- measured on dense products of 4096 channels by
+// 4096 bytes of K, us for (rounds of) workgroups:
+//   few 16 x 16   256: 6.4  512: 10.4  1024: 17.8        tile 64    256: 12.9  512: 19.2  1024: 34.6  2048: 68.0
+//   few 32 x 16   256: 8.3  512: 13.7  1024: 25.1        tile 128   256: 26.4 (4 stages, one workgroup per CU)  512: 51.3
+//   few 32 x 32   256: 10.4 512: 17.6  1024: 31.7        tile 128w  256: 31.7 (2 stages, two per CU)  512: 43.4
+//                                                        tile 256   256: 56 .. 61
+// f32 runs at the f32 matrix rate, a sixteenth of the others': larger tiles gain less there.  The form with the least such cost is
+// taken; sums of 8-bit products are the same by every form.
+enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, TILE128W, TILE256, FORMS };
+struct FormCost {
+    int bm, bn, slots;  // tile, workgroups per round
+    float cost, cost_f32;
+};
+constexpr FormCost FORM[FORMS] = {{16, 16, 256, 3.7f, 3.7f}, {32, 16, 256, 5.5f, 5.4f}, {32, 32, 256, 7.4f, 8.5f}, {64, 64, 256, 8.6f, 19.5f},
+                                  {128, 128, 256, 24.f, 65.f}, {128, 128, 512, 40.f, 127.f}, {256, 256, 256, 56.f, 1e9f}};
+
+// row tiles of bm rows: what the groups can have at most (every group but one may end inside a tile) ...
+long most_row_tiles(const LinearArgs &a, long bm) {
+    return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm;
 }
-template <int T, int MT, int NT, int NW>
-void launch_few(const LinearArgs &a, bool aligned, long m_tiles, hipStream_t s) {
-    const dim3 grid((unsigned)((m_tiles * a.n_tiles + 7) / 8 * 8)), block(64 * NW);
-    if (aligned) hipLaunchKernelGGL((k_linear_few<T, MT, NT, NW, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_linear_few<T, MT, NT, NW, false>), grid, block, 0, s, a);
+// ... and have if the rows are spread evenly
+long even_row_tiles(const LinearArgs &a, long bm) {
+    const long g = std::min(a.groups, a.m), rows = (a.m + g - 1) / g;
+    return g * ((rows + bm - 1) / bm);
 }
 
-template <int T>
+Form pick_form(const LinearArgs &a, bool f32) {
+    int best = FEW11;
+    float least = 3.4e38f;
+    for (int f = 0; f < FORMS; ++f) {
+        const long tiles = even_row_tiles(a, FORM[f].bm) * ((a.n + FORM[f].bn - 1) / FORM[f].bn);
+        const float c = (float)((tiles + FORM[f].slots - 1) / FORM[f].slots) * (f32 ? FORM[f].cost_f32 : FORM[f].cost);
+        if (c < least) {
+            least = c;
+            best = f;
+        }
+    }
+    return (Form)best;
+}
+
+template <int T, bool ALIGNED>
 int launch(LinearArgs a, hipStream_t s) {
-    const bool aligned = !misaligned(a.x, 16) && !misaligned(a.w, 16) && a.ldx % 16 == 0 && a.ldw % 16 == 0;
-    // tiles of BM rows that the groups can have: every group but the largest may end inside one
-    auto m_tiles = [&](long bm) { return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm; };
-    auto n_tiles = [&](long bn) { return (a.n + bn - 1) / bn; };
-    const long mt64 = m_tiles(64) , mt16 = m_tiles(16);
-    const long tiles64 = mt64 * n_tiles(64);
-    if (a.m / a.groups >= 32 && tiles64 >= 192) {
-        a.n_tiles = (int)n_tiles(64);
-        PB_CHECK(mt64 * a.n_tiles < INT_MAX - 8, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
-        launch_tile<T, 64, 64, 32, 32>(a, aligned, mt64, s);
-    } else {
-        a.n_tiles = (int)n_tiles(16);
-        PB_CHECK(mt16 * a.n_tiles < INT_MAX - 8, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
-        launch_few<T, 1, 1, 8>(a, aligned, mt16, s);
+    const Form f = pick_form(a, T == F32);
+    const long row_tiles = most_row_tiles(a, FORM[f].bm), n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
+    PB_CHECK(row_tiles < (INT_MAX - 8) / n_tiles, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
+    a.n_tiles = (int)n_tiles;
+    const dim3 grid((unsigned)((row_tiles * n_tiles + 7) / 8 * 8));
+    switch (f) {
+        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
+        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
+        case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2, ALIGNED>), grid, dim3(512), 0, s, a); break;
+        case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, 4, ALIGNED>), grid, dim3(256), 0, s, a); break;
+        case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
+        case TILE128W: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 64, 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
+        default:
+            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_tile<T, 256, 256, 128, 64, 2, ALIGNED>), grid, dim3(512), 0, s, a);
+            break;
     }
     PB_HIP(hipGetLastError());
     return PB_OK;
+}
+template <int T>
+int launch(const LinearArgs &a, hipStream_t s) {
+    const bool aligned = !misaligned(a.x, 16) && !misaligned(a.w, 16) && a.ldx % 16 == 0 && a.ldw % 16 == 0;
+    return aligned ? launch<T, true>(a, s) : launch<T, false>(a, s);
 }
 
 // what pb_linear_i8 and pb_linear_grouped have in common

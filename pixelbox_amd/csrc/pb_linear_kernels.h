@@ -266,159 +266,221 @@ __device__ __forceinline__ int y_row_of(const LinearArgs &a, int r) {
     return (unsigned)v < (unsigned)a.y_total ? v : -1;
 }
 
-// ---- k_linear_tile: a tile of BM rows x BN channels per workgroup, K in steps of 128 bytes through LDS ------------------------------------
-// Two LDS stages: the loads of step i + 1 run under the matrix instructions of step i, one barrier per step.  Rows sit in LDS at a
-// pitch of 128 bytes with their eight 16-byte pieces permuted by the row number's low three bits (piece c at c ^ (row & 7)), which
-// makes the fragment reads (16 bytes from each of 32 rows) free of bank conflicts; the permutation is done by the lanes' GLOBAL
-// addresses, so a wave's eight rows of 128 bytes are still whole lines.  DMA: the loads go straight into LDS (16-byte aligned
-// rows); otherwise through registers, which takes any alignment.  The last, partial step always goes through registers.
-template <int T, int BM, int BN, int WM, int WN, bool DMA>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(const LinearArgs a) {
-    constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN;
-    constexpr int MT = WM / 32, NT = WN / 32;
-    constexpr int STAGE = (BM + BN) * 128;
-    constexpr int JA = BM * 8 / NTHR, JB = BN * 8 / NTHR;  // 16-byte pieces per thread and step
-    constexpr int PITCH = WN + 4;                          // epilogue image of a wave: 32 rows of WN sums
-    constexpr int EPI = NWM * NWN * 32 * PITCH * 4;
-    static_assert(BM * 8 % NTHR == 0 && BN * 8 % NTHR == 0 && NTHR / 8 % 8 == 0, "");
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[(2 * STAGE > EPI ? 2 * STAGE : EPI)];
-    __shared__ int s_xrow[BM], s_yrow[BM];
-    const Tile t = find_tile<BM, 4>(a);
-    if (t.r0 >= t.r1) return;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+// the tile's rows of x and y, and the scales of its x rows
+template <int T, int BM, int NTHR>
+__device__ __forceinline__ void rows_to_lds(const LinearArgs &a, const Tile &t, int tid, int *xrows, int *yrows, float *scales) {
     for (int i = tid; i < BM; i += NTHR) {
         const int r = t.r0 + i;
-        s_xrow[i] = r < t.r1 ? x_row_of(a, r) : -1;
-        s_yrow[i] = r < t.r1 ? y_row_of(a, r) : -1;
+        int xr = -1, yr = -1;
+        if (r < t.r1) {
+            xr = x_row_of(a, r);
+            yr = xr < 0 ? -1 : y_row_of(a, r);
+        }
+        xrows[i] = xr;
+        yrows[i] = yr;
+        if constexpr (T == I8) scales[i] = xr < 0 ? 0.0f : a.x_scale[xr];
     }
-    __syncthreads();
-    const int lc = (tid & 7) ^ ((tid >> 3) & 7);  // the 16-byte piece this thread moves in every row it touches
-    const uint8_t *pa[JA], *pb[JB];
-#pragma unroll
-    for (int j = 0; j < JA; ++j) pa[j] = a.x + (long)max(s_xrow[(tid + j * NTHR) >> 3], 0) * a.ldx;
-    const int c_base = t.nt * BN;
-#pragma unroll
-    for (int j = 0; j < JB; ++j) pb[j] = a.w + ((long)t.g * a.n + min(c_base + ((tid + j * NTHR) >> 3), a.n - 1)) * a.ldw;
-    const long full = a.kb >> 7, steps = (a.kb + 127) >> 7;
+}
 
-    u32x4 ra[JA], rb[JB];
-    auto load_regs = [&](long i) {
-        const long at = i * 128 + lc * 16;
-        if (i < full) {
-#pragma unroll
-            for (int j = 0; j < JA; ++j) ra[j] = load16<DMA>(pa[j] + at);
-#pragma unroll
-            for (int j = 0; j < JB; ++j) rb[j] = load16<DMA>(pb[j] + at);
-        } else {
-#pragma unroll
-            for (int j = 0; j < JA; ++j) ra[j] = load16_tail<DMA>(pa[j], at, a.kb);
-#pragma unroll
-            for (int j = 0; j < JB; ++j) rb[j] = load16_tail<DMA>(pb[j], at, a.kb);
-        }
-    };
-    auto put_regs = [&](int buf) {
-        uint8_t *s = s_mem + buf * STAGE;
-#pragma unroll
-        for (int j = 0; j < JA; ++j) *reinterpret_cast<u32x4 *>(s + (tid + j * NTHR) * 16) = ra[j];
-#pragma unroll
-        for (int j = 0; j < JB; ++j) *reinterpret_cast<u32x4 *>(s + BM * 128 + (tid + j * NTHR) * 16) = rb[j];
-    };
-    auto dma = [&](long i, int buf) {
-        uint8_t *s = s_mem + buf * STAGE + wave * 1024;  // a wave's 64 lanes fill 1 KiB from here
-        const long at = i * 128 + lc * 16;
-#pragma unroll
-        for (int j = 0; j < JA; ++j)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pa[j] + at),
-                                             (__attribute__((address_space(3))) void *)(s + j * NTHR * 16), 16, 0, 0);
-#pragma unroll
-        for (int j = 0; j < JB; ++j)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pb[j] + at),
-                                             (__attribute__((address_space(3))) void *)(s + BM * 128 + j * NTHR * 16), 16, 0, 0);
-    };
-    const int wm = wave / NWN * WM, wn = wave % NWN * WN;
-    const int li = lane & 31, hi = lane >> 5;
-    typename Acc<T>::q16 acc[NT][MT] = {};
-    auto compute = [&](int buf) {
-        const uint8_t *sa = s_mem + buf * STAGE + (wm + li) * 128, *sb = s_mem + buf * STAGE + (BM + wn + li) * 128;
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            const int c = ((ks * 2 + hi) ^ (li & 7)) * 16;
-            u32x4 fa[MT], fb[NT];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) fb[j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) fa[i] = *reinterpret_cast<const u32x4 *>(sa + i * 4096 + c);
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < MT; ++i) mma32<T>(acc[j][i], fb[j], fa[i]);
-        }
-    };
-    if constexpr (DMA) {
-        auto fetch = [&](long i, int buf) {
-            if (i < full) dma(i, buf);
-            else {
-                load_regs(i);
-                put_regs(buf);
-            }
-        };
-        if (steps > 0) fetch(0, 0);
-        for (long i = 0; i < steps; ++i) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's loads of step i have landed in LDS
-            __syncthreads();                                  // everyone's have, and everyone is done with the other stage
-            if (i + 1 < steps) fetch(i + 1, (int)(i + 1) & 1);
-            compute((int)i & 1);
-        }
-    } else {
-        if (steps > 0) {
-            load_regs(0);
-            put_regs(0);
-        }
-        for (long i = 0; i < steps; ++i) {
-            __syncthreads();
-            if (i + 1 < steps) load_regs(i + 1);
-            compute((int)i & 1);
-            if (i + 1 < steps) put_regs((int)(i + 1) & 1);
-        }
-    }
-    __syncthreads();  // the stages become the waves' epilogue images
-    // a wave turns 32 rows x WN channels at a time: its sums go to LDS as the matrix instruction left them (4 consecutive channels
-    // per lane) and come back as 8 consecutive channels per lane, whole rows by consecutive lanes
+// A wave's sums -> y, 32 rows x WN channels at a time: they go to LDS as the matrix instruction left them (4 consecutive channels per
+// lane) and come back as 8 consecutive channels per lane, whole rows by consecutive lanes.  s_mem: 32 (WN + 4) sums for each wave.
+template <int T, int MT, int NT, int WN>
+__device__ __forceinline__ void store_tile(const LinearArgs &a, int g, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem, const int *yrows,
+                                           const float *scales, int wave, int lane, int c_wave) {
     typedef typename Acc<T>::e E;
+    typedef typename Acc<T>::q4 Q;
+    constexpr int PITCH = WN + 4;
     E *img = reinterpret_cast<E *>(s_mem) + wave * 32 * PITCH;
     constexpr int LPR = WN / 8, RPI = 64 / LPR;  // lanes per row, rows per instruction
-    const int c8 = (lane % LPR) * 8, c0 = c_base + wn + c8;
-    const Chan<T, 8> ch(a, t.g, c0);
+    const int li = lane & 31, hi = lane >> 5;
+    const int c8 = (lane % LPR) * 8, c0 = c_wave + c8;
+    const Chan<T, 8> ch(a, g, c0);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                typename Acc<T>::q4 v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-                *reinterpret_cast<typename Acc<T>::q4 *>(img + li * PITCH + j * 32 + q * 8 + hi * 4) = v;
+                const Q v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+                *reinterpret_cast<Q *>(img + li * PITCH + j * 32 + q * 8 + hi * 4) = v;
             }
         __builtin_amdgcn_wave_barrier();  // one wave's LDS accesses are in order
 #pragma unroll
         for (int r = lane / LPR; r < 32; r += RPI) {
-            const int at = wm + i * 32 + r, yr = s_yrow[at], xr = s_xrow[at];
-            const typename Acc<T>::q4 lo = *reinterpret_cast<const typename Acc<T>::q4 *>(img + r * PITCH + c8);
-            const typename Acc<T>::q4 up = *reinterpret_cast<const typename Acc<T>::q4 *>(img + r * PITCH + c8 + 4);
+            const int yr = yrows[i * 32 + r];
+            const Q lo = *reinterpret_cast<const Q *>(img + r * PITCH + c8), up = *reinterpret_cast<const Q *>(img + r * PITCH + c8 + 4);
             const E s[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-            if (yr >= 0 && xr >= 0) ch.finish(a, s, T == I8 ? a.x_scale[xr] : 1.0f, yr, c0);
+            if (yr >= 0) ch.finish(a, s, T == I8 ? scales[i * 32 + r] : 1.0f, yr, c0);
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
+// ---- k_linear_tile: a tile of BM rows x BN channels per workgroup, K in steps of 128 bytes through LDS ------------------------------------
+// A step has four pieces of 32 bytes of K; a piece's fragments are read from LDS while the one before is multiplied.  The one barrier
+// of a step stands before its LAST piece, whose fragments are in registers by then: behind it the step's stage is free, so the loads
+// of step i + NST leave there (NST LDS stages) and have NST - 1 steps to arrive, and the first fragments of step i + 1 are read while
+// the last piece of step i is multiplied -- the matrix pipe has work across the barrier.  Waves with one or two matrix instructions
+// to a piece (FLAT) would wait out an LDS read for each piece: they read all four at once behind the barrier.
+// Rows sit in LDS at a pitch of 128 bytes with their eight 16-byte pieces permuted (piece c at c ^ (row / 2 & 7)), which makes the
+// fragment reads (16 bytes from each of 32 rows) free of bank conflicts: 249 bytes a clock and CU, against 121 with c ^ (row & 7)
+// and 32 unpermuted (LDS reads alone, 256 workgroups of eight waves); the permutation is done by the lanes' GLOBAL addresses, so a
+// wave's eight rows of 128 bytes are still whole lines.  DMA: the loads go straight into LDS (16-byte aligned rows); otherwise
+// through registers, which takes any alignment.  The last, partial step always goes through registers.
+template <int T, int BM, int BN, int WM, int WN, int NST, bool DMA>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(const LinearArgs a) {
+    constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN;
+    constexpr int MT = WM / 32, NT = WN / 32;
+    constexpr int STAGE = (BM + BN) * 128;
+    constexpr int JA = BM * 8 / NTHR, J = (BM + BN) * 8 / NTHR;  // 16-byte pieces per thread and step: of x, in all
+    constexpr int PITCH = WN + 4;                                // epilogue image of a wave: 32 rows of WN sums
+    constexpr int EPI = NWM * NWN * 32 * PITCH * 4;
+    constexpr bool FLAT = MT * NT <= 2;
+    constexpr int NF = FLAT ? 4 : 2;  // pieces held in registers
+    static_assert(BM * 8 % NTHR == 0 && BN * 8 % NTHR == 0 && NTHR / 8 % 16 == 0 && (NST == 2 || NST == 4), "");
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[(NST * STAGE > EPI ? NST * STAGE : EPI)];
+    __shared__ int s_xrow[BM], s_yrow[BM];
+    __shared__ float s_scale[T == I8 ? BM : 1];
+    const Tile t = find_tile<BM, 4>(a);
+    if (t.r0 >= t.r1) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    rows_to_lds<T, BM, NTHR>(a, t, tid, s_xrow, s_yrow, s_scale);
+    __syncthreads();
+    const int lc = ((tid & 7) ^ ((tid >> 4) & 7)) * 16;  // the 16-byte piece this thread moves in every row it touches
+    const int c_base = t.nt * BN;
+    const uint8_t *pp[J];  // its rows: JA of x, the others of w
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int row = ((tid + j * NTHR) >> 3);
+        pp[j] = (j < JA ? a.x + (long)max(s_xrow[j < JA ? row : 0], 0) * a.ldx : a.w + ((long)t.g * a.n + min(c_base + row - BM, a.n - 1)) * a.ldw) + lc;
+    }
+    const int full = (int)(a.kb >> 7), steps = (int)((a.kb + 127) >> 7);
+    auto stage = [&](int i) { return s_mem + (i & (NST - 1)) * STAGE; };
+    auto dma = [&](int i, int j) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pp[j] + (long)i * 128),
+                                         (__attribute__((address_space(3))) void *)(stage(i) + wave * 1024 + j * NTHR * 16), 16, 0, 0);
+    };
+    auto copy_tail = [&](int i) {  // the partial step behind the full ones
+#pragma unroll 1
+        for (int j = 0; j < J; ++j) {
+            const uint8_t *row = j < JA ? a.x + (long)max(s_xrow[(tid + j * NTHR) >> 3], 0) * a.ldx
+                                        : a.w + ((long)t.g * a.n + min(c_base + ((tid + j * NTHR) >> 3) - BM, a.n - 1)) * a.ldw;
+            *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = load16_tail<DMA>(row, (long)i * 128 + lc, a.kb);
+        }
+    };
+    u32x4 regs[DMA ? 1 : J];
+    auto load_regs = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) regs[DMA ? 0 : j] = load16<false>(pp[j] + (long)i * 128);
+    };
+    auto put_regs = [&](int i) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = regs[DMA ? 0 : j];
+    };
+    const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 31, hi = lane >> 5;
+    typename Acc<T>::q16 acc[NT][MT] = {};
+    const uint8_t *sa = s_mem + (wm + li) * 128, *sb = s_mem + (BM + wn + li) * 128;
+    u32x4 fa[NF][MT], fb[NF][NT];
+    auto read = [&](int i, int ks, int to) {
+        const int c = (i & (NST - 1)) * STAGE + ((ks * 2 + hi) ^ ((li >> 1) & 7)) * 16;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) fb[to][j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) fa[to][m] = *reinterpret_cast<const u32x4 *>(sa + m * 4096 + c);
+    };
+    // a piece; `send`: the loads of step i among its matrix instructions
+    auto multiply = [&](int from, bool send, int i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma32<T>(acc[j][m], fb[from][j], fa[from][m]);
+            if constexpr (DMA) {
+                if (send) {
+#pragma unroll
+                    for (int l = j * J / NT; l < (j + 1) * J / NT; ++l) dma(i, l);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // this wave's loads of step i are in LDS; those of younger steps may still be on their way
+    auto landed = [&](int i) {
+        const int younger = min(NST - 2, full - 1 - i);
+        if (NST > 3 && younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * J) : "memory");
+        else if (NST > 2 && younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    for (int i = 0; i < NST; ++i) {
+        if (i < full) {
+            if constexpr (DMA) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) dma(i, j);
+            } else {
+                load_regs(i);
+                put_regs(i);
+            }
+        } else if (i < steps) copy_tail(i);
+    }
+    auto barrier = [&] {  // this wave's LDS reads have come back, its LDS writes are done
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if constexpr (FLAT) {
+        for (int i = 0; i < steps; ++i) {
+            landed(i);
+            barrier();  // step i is in LDS, everyone has read step i - 1
+            const int next = i - 1 + NST;
+            const bool more = i > 0 && next < full;
+            if (more) {
+                if constexpr (DMA) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) dma(next, j);
+                } else load_regs(next);
+            } else if (i > 0 && next == full && full < steps) copy_tail(full);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) read(i, ks, ks);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) multiply(ks, false, 0);
+            if constexpr (!DMA) {
+                if (more) put_regs(next);
+            }
+        }
+    } else {
+        landed(0);
+        barrier();
+        if (steps > 0) read(0, 0, 0);
+        for (int i = 0; i < steps; ++i) {
+            const bool more = !DMA && i > 0 && i + NST - 1 < full;
+            if (more) load_regs(i + NST - 1);
+            read(i, 1, 1);
+            multiply(0, false, 0);
+            read(i, 2, 0);
+            multiply(1, false, 0);
+            read(i, 3, 1);
+            multiply(0, false, 0);
+            if (more) put_regs(i + NST - 1);
+            landed(i + 1);
+            barrier();  // the last piece's fragments are in registers everywhere, step i + 1 is in LDS
+            if (i + NST == full && full < steps) copy_tail(full);
+            if (i + 1 < steps) read(i + 1, 0, 0);
+            multiply(1, DMA && i + NST < full, i + NST);
+        }
+    }
+    __syncthreads();  // the stages become the waves' epilogue images
+    store_tile<T, MT, NT, WN>(a, t.g, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn);
+}
+
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
 // For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
 // waves' partial sums meet in LDS and are added in wave order.
-template <int T, int MT, int NT, int NW, bool ALIGNED>
+template <int T, int MT, int NT, int NW, int U, bool ALIGNED>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     typedef typename Acc<T>::e E;
     typedef typename Acc<T>::q4 Q;
-    constexpr int BM = 16 * MT, BN = 16 * NT, U = 4;
+    constexpr int BM = 16 * MT, BN = 16 * NT;
     constexpr int PITCH = BN + 4;
     __shared__ __attribute__((aligned(16))) E s_sum[NW][BM * PITCH];
     const Tile t = find_tile<BM, 1>(a);

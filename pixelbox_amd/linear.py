@@ -24,22 +24,31 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 _ACTS = {"none": capi.PB_ACT_NONE, "silu": capi.PB_ACT_SILU, "tanh": capi.PB_ACT_TANH}
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# the current stream's handle without making a Stream object: 0.1 us a call instead of 1.7
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _device(t: torch.Tensor, name: str) -> torch.device:
-    if t.device.type != "cuda":
+def _stream(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _device(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
         raise ValueError(f"{name} is on {t.device}: the operators run on a GPU")
-    return t.device
+    return index
 
 
-def _check(t: torch.Tensor, name: str, shape: tuple, dtypes, device: torch.device) -> None:
-    """dtype, device, shape (None: any length) and a contiguous last axis; rows do not overlap one another"""
+# One call of these operators is a kernel of a few microseconds, so the usual tensor -- right type, shape and device, contiguous -- passes in
+# one comparison each; only what fails it is looked at closely.
+def _check(t: torch.Tensor, name: str, shape: tuple, dtypes: tuple, index: int) -> None:
+    """dtype, device, shape (None: any length) and a contiguous last axis"""
+    if t.dtype in dtypes and t.get_device() == index and t.shape == shape and t.is_contiguous():
+        return
     if t.dtype not in dtypes:
         raise TypeError(f"{name} is {t.dtype}, not {' or '.join(str(d) for d in dtypes)}")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other tensors are on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, x is on GPU {index}")
     if t.dim() != len(shape) or any(want is not None and have != want for have, want in zip(t.shape, shape)):
         raise ValueError(f"{name} has the shape {tuple(t.shape)}, not {shape}")
     if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
@@ -49,7 +58,7 @@ def _check(t: torch.Tensor, name: str, shape: tuple, dtypes, device: torch.devic
 def _ld(t: torch.Tensor, name: str) -> int:
     """distance between the rows of a 2-d tensor"""
     n = t.shape[1]
-    if t.shape[0] <= 1:
+    if t.is_contiguous() or t.shape[0] <= 1:
         return n
     ld = t.stride(0)
     if ld < n:
@@ -58,7 +67,11 @@ def _ld(t: torch.Tensor, name: str) -> int:
 
 
 def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if not torch.is_grad_enabled():
+        return
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
         raise ValueError("these products have no gradient: an operand requires one (detach it, or call under torch.no_grad())")
 
 
@@ -81,19 +94,21 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scale: tor
     """x [m, k] (f32, bf16, f16) -> (codes int8 [m, k], scale f32 [m]): scale = max(max |x| / 127, 2^-126) of each row, codes rounded to the
     nearest, halves to even.  A row with an infinity or a NaN has scale NaN and codes 0."""
     dev = _device(x, "x")
-    _check(x, "x", (None, None), _FLOATS, dev)
-    _no_grad(x)
+    if x.dim() != 2:
+        raise ValueError(f"x has the shape {tuple(x.shape)}, not (rows, values)")
     m, k = x.shape
+    _check(x, "x", (m, k), _FLOATS, dev)
+    _no_grad(x)
     if codes is None:
-        codes = torch.empty((m, k), dtype=torch.int8, device=dev)
+        codes = torch.empty((m, k), dtype=torch.int8, device=x.device)
     else:
         _check(codes, "codes", (m, k), (torch.int8,), dev)
     if scale is None:
-        scale = torch.empty((m,), dtype=torch.float32, device=dev)
+        scale = torch.empty((m,), dtype=torch.float32, device=x.device)
     else:
         _check(scale, "scale", (m,), (torch.float32,), dev)
     ldx, ldc = _ld(x, "x"), _ld(codes, "codes")
-    _call(capi.lib().pb_quantize_rows(dev.index, _stream(dev), x.data_ptr(), _TYPES[x.dtype], m, k, ldx, codes.data_ptr(), ldc, scale.data_ptr()))
+    _call(capi.lib().pb_quantize_rows(dev, _stream(dev), x.data_ptr(), _TYPES[x.dtype], m, k, ldx, codes.data_ptr(), ldc, scale.data_ptr()))
     return codes, scale
 
 
@@ -103,23 +118,25 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     `dtype`, or out's."""
     dev = _device(x, "x")
     code = _act(act)
-    _check(x, "x", (None, None), (torch.int8,), dev)
+    if x.dim() != 2 or w.dim() != 2:
+        raise ValueError(f"x and w have the shapes {tuple(x.shape)} and {tuple(w.shape)}, not (m, k) and (n, k)")
     m, k = x.shape
-    _check(w, "w", (None, k), (torch.int8,), dev)
     n = w.shape[0]
+    _check(x, "x", (m, k), (torch.int8,), dev)
+    _check(w, "w", (n, k), (torch.int8,), dev)
     _check(x_scale, "x_scale", (m,), (torch.float32,), dev)
     _check(w_scale, "w_scale", (n,), (torch.float32,), dev)
     if bias is not None:
         _check(bias, "bias", (n,), (torch.float32,), dev)
-    _no_grad(x_scale, w_scale, bias)
+    _no_grad(x_scale, w_scale, bias, out)
     if out is None:
         if dtype not in _FLOATS:
             raise TypeError(f"dtype is {dtype}, not one of {', '.join(str(d) for d in _FLOATS)}")
-        out = torch.empty((m, n), dtype=dtype, device=dev)
+        out = torch.empty((m, n), dtype=dtype, device=x.device)
     else:
         _check(out, "out", (m, n), _FLOATS, dev)
     ldx, ldw, ldy = _ld(x, "x"), _ld(w, "w"), _ld(out, "out")
-    _call(capi.lib().pb_linear_i8(dev.index, _stream(dev), x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), code,
+    _call(capi.lib().pb_linear_i8(dev, _stream(dev), x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), code,
                                   out.data_ptr(), _TYPES[out.dtype], ldy, m, n, k))
     return out
 
@@ -128,19 +145,21 @@ def group_rows(group: torch.Tensor, groups: int, offsets: torch.Tensor | None = 
     """group int32 [m] -> (offsets int32 [groups + 1], order int32 [m]): group g's rows are order[offsets[g] : offsets[g + 1]], ascending.  Rows with a
     group outside [0, groups) come last, behind offsets[groups]."""
     dev = _device(group, "group")
-    _check(group, "group", (None,), (torch.int32,), dev)
+    if group.dim() != 1:
+        raise ValueError(f"group has the shape {tuple(group.shape)}, not (rows,)")
     m = group.shape[0]
+    _check(group, "group", (m,), (torch.int32,), dev)
     if not 1 <= groups <= capi.PB_MAX_GROUPS:
         raise ValueError(f"groups is {groups}, not 1 .. {capi.PB_MAX_GROUPS}")
     if offsets is None:
-        offsets = torch.empty((groups + 1,), dtype=torch.int32, device=dev)
+        offsets = torch.empty((groups + 1,), dtype=torch.int32, device=group.device)
     else:
         _check(offsets, "offsets", (groups + 1,), (torch.int32,), dev)
     if order is None:
-        order = torch.empty((m,), dtype=torch.int32, device=dev)
+        order = torch.empty((m,), dtype=torch.int32, device=group.device)
     else:
         _check(order, "order", (m,), (torch.int32,), dev)
-    _call(capi.lib().pb_group_rows(dev.index, _stream(dev), group.data_ptr(), m, groups, offsets.data_ptr(), order.data_ptr()))
+    _call(capi.lib().pb_group_rows(dev, _stream(dev), group.data_ptr(), m, groups, offsets.data_ptr(), order.data_ptr()))
     return offsets, order
 
 
@@ -155,29 +174,33 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     where y_rows is given)."""
     dev = _device(x, "x")
     code = _act(act)
-    _check(x, "x", (None, None), _FLOATS + (torch.int8,), dev)
+    if x.dim() != 2 or w.dim() != 3:
+        raise ValueError(f"x and w have the shapes {tuple(x.shape)} and {tuple(w.shape)}, not (rows, k) and (groups, n, k)")
     x_total, k = x.shape
-    if w.dim() != 3:
-        raise ValueError(f"w has the shape {tuple(w.shape)}, not (groups, n, k)")
     groups, n, _ = w.shape
-    _check(w, "w", (None, None, k), (x.dtype,), dev)
+    _check(x, "x", (x_total, k), _FLOATS + (torch.int8,), dev)
+    _check(w, "w", (groups, n, k), (x.dtype,), dev)
     if not 1 <= groups <= capi.PB_MAX_GROUPS:
         raise ValueError(f"w has {groups} groups, not 1 .. {capi.PB_MAX_GROUPS}")
-    ldw = w.stride(1) if n > 1 else k
-    if ldw < k or (groups > 1 and n > 0 and w.stride(0) != n * ldw):
-        raise ValueError("w: the groups' weights do not follow one another row by row")
+    ldw = k
+    if not w.is_contiguous():
+        ldw = w.stride(1) if n > 1 else w.stride(0) if n == 1 and groups > 1 else k
+        if ldw < k or (groups > 1 and n > 0 and w.stride(0) != n * ldw):
+            raise ValueError("w: the groups' weights do not follow one another row by row")
     _check(offsets, "offsets", (groups + 1,), (torch.int32,), dev)
     if rows is not None:
         if x_rows is not None or y_rows is not None:
             raise ValueError("rows stands for x_rows and y_rows: give one or the other")
         x_rows = y_rows = rows
     m = x_total
-    for t, name in ((x_rows, "x_rows"), (y_rows, "y_rows")):
-        if t is not None:
-            _check(t, name, (None,), (torch.int32,), dev)
-            m = t.shape[0]
-    if x_rows is not None and y_rows is not None and x_rows.shape[0] != y_rows.shape[0]:
-        raise ValueError(f"x_rows and y_rows differ in length: {x_rows.shape[0]}, {y_rows.shape[0]}")
+    if x_rows is not None:
+        m = x_rows.numel()
+        _check(x_rows, "x_rows", (m,), (torch.int32,), dev)
+    if y_rows is not None and y_rows is not x_rows:
+        m = y_rows.numel()
+        _check(y_rows, "y_rows", (m,), (torch.int32,), dev)
+        if x_rows is not None and x_rows.shape[0] != m:
+            raise ValueError(f"x_rows and y_rows differ in length: {x_rows.shape[0]}, {m}")
     if x_rows is None and m > x_total:
         raise ValueError(f"y_rows lists {m} rows, x has {x_total}")
     i8 = x.dtype == torch.int8
@@ -191,22 +214,22 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     if bias is not None:
         _check(bias, "bias", (groups, n), (torch.float32,), dev)
     for t, name in ((w_scale, "w_scale"), (bias, "bias")):
-        if t is not None and groups > 1 and n > 0 and t.stride(0) != n:
+        if t is not None and not t.is_contiguous():
             raise ValueError(f"{name}: the groups' rows do not follow one another")
-    _no_grad(x, w, x_scale, w_scale, bias)
+    _no_grad(x, w, x_scale, w_scale, bias, out)
     if out is None:
         dtype = dtype or (torch.float32 if i8 else x.dtype)
         if dtype not in _FLOATS:
             raise TypeError(f"dtype is {dtype}, not one of {', '.join(str(d) for d in _FLOATS)}")
-        out = torch.zeros((m if y_rows is None else max(m, x_total), n), dtype=dtype, device=dev)
+        out = torch.zeros((m if y_rows is None else max(m, x_total), n), dtype=dtype, device=x.device)
     else:
-        _check(out, "out", (None, n), _FLOATS, dev)
+        _check(out, "out", (out.shape[0] if out.dim() else 0, n), _FLOATS, dev)
         if y_rows is None and out.shape[0] < m:
             raise ValueError(f"out has {out.shape[0]} rows, {m} may be written")
     if m == 0 or n == 0 or (out.shape[0] == 0 and y_rows is not None) or x_total == 0:
         return out
     ldx, ldy = _ld(x, "x"), _ld(out, "out")
-    _call(capi.lib().pb_linear_grouped(dev.index, _stream(dev), _TYPES[x.dtype], x.data_ptr(), x_total, ldx, _ptr(x_scale), w.data_ptr(), ldw,
+    _call(capi.lib().pb_linear_grouped(dev, _stream(dev), _TYPES[x.dtype], x.data_ptr(), x_total, ldx, _ptr(x_scale), w.data_ptr(), ldw,
                                        _ptr(w_scale), _ptr(bias), offsets.data_ptr(), groups, _ptr(x_rows), _ptr(y_rows), code, out.data_ptr(),
                                        _TYPES[out.dtype], out.shape[0], ldy, m, n, k))
     return out

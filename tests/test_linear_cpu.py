@@ -89,6 +89,9 @@ class _Fake(torch.Tensor):
     def device(self):
         return torch.device("cuda", self.__dict__.get("at", 0))
 
+    def get_device(self):
+        return self.__dict__.get("at", 0)
+
 
 def fake(t, at=0):
     f = t.as_subclass(_Fake)

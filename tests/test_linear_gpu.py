@@ -127,6 +127,40 @@ def test_linear_i8(m, n, k):
         ref.check(y, *ref.linear(x, w, bias, name, dt, xs, ws), (m, n, k, name))
 
 
+# sizes that each form of the product is chosen for (16 x 16, 32 x 16 and 32 x 32 outputs per workgroup with K split over its waves; tiles of 64,
+# 128 with four and with two LDS stages, 256), K around whole steps of 128 bytes and around the stages' number, rows on 16 bytes and not
+FORM_SIZES = [(16, 4096), (32, 4096), (60, 4000), (300, 1000), (1000, 4000), (2048, 4090), (4000, 4096)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n", FORM_SIZES)
+def test_every_form_at_every_remainder(kind, m, n):
+    size = {"f32": 4, "bf16": 2, "f16": 2, "i8": 1}[kind]
+    most = 1040 // size
+    x, xs, w, ws, b = grouped_case(kind, m, 1, n, most, m + n)
+    offsets = torch.tensor([0, m], dtype=torch.int32).cuda()
+    rows = gen(3)
+    pick = torch.randperm(m, generator=rows)[:70]  # rows that are compared with 64 bits; all are compared with one another's K below
+    for k in [most, 512 // size, 512 // size + 1, 640 // size - 1, 128 // size, 128 // size + 3, 256 // size, 5]:
+        xk, wk = x[:, :k], w[:, :, :k]
+        if k == most - 0:
+            xk, wk = x, w
+        if k % 2:
+            xk, wk = xk.contiguous(), wk.contiguous()
+        y = torch.full((m, n), float("nan"), device="cuda")
+        linear.linear_grouped(xk, wk, offsets, x_scale=xs, w_scale=ws, bias=b, out=y)
+        assert not torch.isnan(y).any(), k
+        ref.check(y[pick.cuda()], *ref.linear(x.cpu()[pick][:, :k], w[0, :, :k], b[0], "none", torch.float32, None if xs is None else xs.cpu()[pick],
+                                              None if ws is None else ws[0]), (m, n, k))
+        # every row and channel against the same product on the GPU in 64 bits: order of sums aside, the same
+        want = x[:, :k].double() @ w[0, :, :k].double().t()
+        if kind == "i8":
+            want = want * xs.double()[:, None] * ws[0].double()
+        want += b[0].double()
+        scale = want.abs().amax().item()
+        assert (y.double() - want).abs().amax().item() <= 2e-5 * scale
+
+
 def test_linear_i8_sums_are_exact_at_the_largest_k():
     k = capi.PB_LINEAR_I8_MAX_K
     x = torch.full((2, k), -128, dtype=torch.int8, device="cuda")
