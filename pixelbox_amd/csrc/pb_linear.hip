@@ -5,6 +5,7 @@
 // holds nothing that another one shares.
 #include <algorithm>
 #include <climits>
+#include <cmath>
 
 #include "pb_common.h"
 #include "pb_linear_kernels.h"
@@ -48,35 +49,39 @@ constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 
 //   few 32 x 16   256: 8.3  512: 13.7  1024: 25.1        tile 128   256: 26.4 (4 stages, one workgroup per CU)  512: 51.3
 //   few 32 x 32   256: 10.4 512: 17.6  1024: 31.7        tile 128w  256: 31.7 (2 stages, two per CU)  512: 43.4
 //                                                        tile 256   256: 56 .. 61
-// f32 runs at the f32 matrix rate, a sixteenth of the others': larger tiles gain less there.  The form with the least such cost is
-// taken; sums of 8-bit products are the same by every form.
+// A tile that holds next to no rows costs the few forms less (`thin`; 1 x 4096: 5.1 against 6.4; 32 rows over 64 groups, 2048 x 2048
+// bf16: 16 x 16 32 us, 32 x 32 50, tile 64 42).  f32 runs at the f32 matrix rate, a sixteenth of the others': larger tiles gain less there.  Rows off 16 bytes cost the
+// few forms twice and more (16 x 4096 x 4099: 14.1 us, tile 64 18.6; 64 rows: 24.3, 21.6), the tiles a third to a half.  The form with
+// the least such cost is taken; sums of 8-bit products are the same by every form.
 enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, TILE128W, TILE256, FORMS };
 struct FormCost {
     int bm, bn, slots;  // tile, workgroups per round
-    float cost, cost_f32;
+    float cost, cost_f32, cost_off, thin;
 };
-constexpr FormCost FORM[FORMS] = {{16, 16, 256, 3.7f, 3.7f}, {32, 16, 256, 5.5f, 5.4f}, {32, 32, 256, 7.4f, 8.5f}, {64, 64, 256, 8.6f, 19.5f},
-                                  {128, 128, 256, 24.f, 65.f}, {128, 128, 512, 40.f, 127.f}, {256, 256, 256, 56.f, 1e9f}};
+constexpr FormCost FORM[FORMS] = {{16, 16, 256, 3.7f, 3.7f, 11.f, 0.48f},  {32, 16, 256, 5.5f, 5.4f, 16.f, 0.8f}, {32, 32, 256, 7.4f, 8.5f, 20.5f, 0.8f},
+                                  {64, 64, 256, 8.6f, 19.5f, 15.f, 1.f},   {128, 128, 256, 24.f, 65.f, 41.f, 1.f}, {128, 128, 512, 40.f, 127.f, 60.f, 1.f},
+                                  {256, 256, 256, 56.f, 1e9f, 92.f, 1.f}};
 
 // row tiles of bm rows: what the groups can have at most (every group but one may end inside a tile) ...
 long most_row_tiles(const LinearArgs &a, long bm) {
     return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm;
 }
-// ... and have if the rows are spread evenly
-long even_row_tiles(const LinearArgs &a, long bm) {
-    const long g = std::min(a.groups, a.m), rows = (a.m + g - 1) / g;
-    return g * ((rows + bm - 1) / bm);
-}
 
-Form pick_form(const LinearArgs &a, bool f32) {
+Form pick_form(const LinearArgs &a, bool f32, bool aligned) {
+    // ... and will have: the lengths are not known here, a group's last tile is half full in the middle (512 rows over 8 groups of 40
+    // to 110, 256 x 1280 f32: taken as 8 x 2 full tiles of 32 rows the product took 20 us by 32 x 16, by 32 x 32 15)
+    const float groups = (float)std::min(a.groups, a.m), rows = (float)a.m / groups;
     int best = FEW11;
     float least = 3.4e38f;
-    for (int f = 0; f < FORMS; ++f) {
-        const long tiles = even_row_tiles(a, FORM[f].bm) * ((a.n + FORM[f].bn - 1) / FORM[f].bn);
-        const float c = (float)((tiles + FORM[f].slots - 1) / FORM[f].slots) * (f32 ? FORM[f].cost_f32 : FORM[f].cost);
+    for (int i = 0; i < FORMS; ++i) {
+        const FormCost &f = FORM[i];
+        const float per_group = groups > 1 ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)((a.m + f.bm - 1) / f.bm);
+        const float tiles = groups * per_group * (float)((a.n + f.bn - 1) / f.bn);
+        float c = std::ceil(tiles / (float)f.slots) * std::max(f32 ? f.cost_f32 : f.cost, aligned ? 0.f : f.cost_off);
+        c *= f.thin + (1.f - f.thin) * std::min(1.f, rows / (float)f.bm);
         if (c < least) {
             least = c;
-            best = f;
+            best = i;
         }
     }
     return (Form)best;
@@ -84,7 +89,7 @@ Form pick_form(const LinearArgs &a, bool f32) {
 
 template <int T, bool ALIGNED>
 int launch(LinearArgs a, hipStream_t s) {
-    const Form f = pick_form(a, T == F32);
+    const Form f = pick_form(a, T == F32, ALIGNED);
     const long row_tiles = most_row_tiles(a, FORM[f].bm), n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
     PB_CHECK(row_tiles < (INT_MAX - 8) / n_tiles, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
     a.n_tiles = (int)n_tiles;
@@ -93,7 +98,7 @@ int launch(LinearArgs a, hipStream_t s) {
         case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
         case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
         case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2, ALIGNED>), grid, dim3(512), 0, s, a); break;
-        case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, 4, ALIGNED>), grid, dim3(256), 0, s, a); break;
+        case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, ALIGNED ? 4 : 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
         case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
         case TILE128W: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 64, 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
         default:
@@ -118,7 +123,7 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     PB_CHECK(!bad_type(y_type), PB_ERR_INVALID, "%s: unknown output type %d (f32, bf16, f16)", who, y_type);
     PB_CHECK(act >= PB_ACT_NONE && act <= PB_ACT_TANH, PB_ERR_INVALID, "%s: unknown activation %d", who, act);
     PB_CHECK(m <= INT_MAX && x_total <= INT_MAX && y_total <= INT_MAX, PB_ERR_INVALID, "%s: more than 2^31 - 1 rows", who);
-    PB_CHECK(n <= (uint32_t)INT_MAX / 2 && k <= (uint32_t)INT_MAX / 4, PB_ERR_INVALID, "%s: n = %u, k = %u is out of range", who, n, k);
+    PB_CHECK(n <= (uint32_t)INT_MAX / 2 && k <= 1u << 28, PB_ERR_INVALID, "%s: n = %u, k = %u is out of range", who, n, k);
     PB_CHECK(!i8 || k <= PB_LINEAR_I8_MAX_K, PB_ERR_INVALID, "%s: k = %u would overflow 32-bit sums (at most %u)", who, k, PB_LINEAR_I8_MAX_K);
     PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
     PB_CHECK(ldx >= k && ldw >= k && ldy >= n && ldx <= MAX_LD && ldw <= MAX_LD && ldy <= MAX_LD, PB_ERR_INVALID,
@@ -171,11 +176,15 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     }
 }
 
+// a wave per row where the row fits its registers and there are rows for every CU, else a workgroup of four
 template <int T, bool VEC>
-void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, int8_t *codes, uint64_t ldc, float *scale, hipStream_t s) {
+void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale, hipStream_t s) {
     const uint8_t *px = static_cast<const uint8_t *>(x);
-    hipLaunchKernelGGL((k_quantize_rows<T, 256, 4, VEC>), dim3((unsigned)m), dim3(256), 0, s, px, (long)m, (int)k, (long)ldx * type_bytes(T), codes, (long)ldc,
-                       scale);
+    int8_t *pc = static_cast<int8_t *>(codes);
+    constexpr uint32_t V = T == F32 ? 4 : 8;
+    const long lx = (long)ldx * type_bytes(T), lc = (long)ldc;
+    if (m >= 1024 && k <= 64 * V * 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 8, VEC>), dim3((unsigned)((m + 3) / 4)), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
+    else hipLaunchKernelGGL((k_quantize_rows<T, 256, 4, VEC>), dim3((unsigned)m), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
 }
 
 }  // namespace
@@ -185,7 +194,7 @@ extern "C" {
 int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale) {
     const char *who = "pb_quantize_rows";
     PB_CHECK(!bad_type(x_type), PB_ERR_INVALID, "%s: unknown type %d (f32, bf16, f16)", who, x_type);
-    PB_CHECK(m <= INT_MAX && k <= (uint32_t)INT_MAX / 4, PB_ERR_INVALID, "%s: m = %llu, k = %u is out of range", who, (unsigned long long)m, k);
+    PB_CHECK(m <= INT_MAX && k <= 1u << 28, PB_ERR_INVALID, "%s: m = %llu, k = %u is out of range", who, (unsigned long long)m, k);
     PB_CHECK(ldx >= k && ldc >= k && ldx <= MAX_LD && ldc <= MAX_LD, PB_ERR_INVALID, "%s: rows of %u values do not fit their strides", who, k);
     if (m == 0) return PB_OK;
     const int size = type_bytes(x_type);
@@ -199,9 +208,9 @@ int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64
     const int v = x_type == PB_TYPE_F32 ? 4 : 8;
     const bool vec = !misaligned(x, 16) && ldx * size % 16 == 0 && !misaligned(codes, v) && ldc % v == 0;
     switch (x_type) {
-        case PB_TYPE_F32: vec ? launch_quantize<F32, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<F32, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
-        case PB_TYPE_BF16: vec ? launch_quantize<BF16, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<BF16, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
-        default: vec ? launch_quantize<F16, true>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s) : launch_quantize<F16, false>(x, m, k, ldx, static_cast<int8_t *>(codes), ldc, scale, s); break;
+        case PB_TYPE_F32: vec ? launch_quantize<F32, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<F32, false>(x, m, k, ldx, codes, ldc, scale, s); break;
+        case PB_TYPE_BF16: vec ? launch_quantize<BF16, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<BF16, false>(x, m, k, ldx, codes, ldc, scale, s); break;
+        default: vec ? launch_quantize<F16, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<F16, false>(x, m, k, ldx, codes, ldc, scale, s); break;
     }
     PB_HIP(hipGetLastError());
     return PB_OK;
@@ -223,8 +232,10 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
              PB_ERR_INVALID, "%s: buffers overlap", who);
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
-    hipLaunchKernelGGL(k_group_rows, dim3(groups + 1), dim3(64 * GR_WAVES), 0, static_cast<hipStream_t>(stream), group, (int)m, (int)groups,
-                       (int)!misaligned(group, 16), offsets, order);
+    const int vec = !misaligned(group, 16);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (m <= 4096) hipLaunchKernelGGL((k_group_rows<4>), dim3(groups + 1), dim3(256), 0, s, group, (int)m, (int)groups, vec, offsets, order);
+    else hipLaunchKernelGGL((k_group_rows<16>), dim3(groups + 1), dim3(1024), 0, s, group, (int)m, (int)groups, vec, offsets, order);
     PB_HIP(hipGetLastError());
     return PB_OK;
 }

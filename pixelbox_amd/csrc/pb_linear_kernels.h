@@ -10,6 +10,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "pb_embed_common.h"
 
 namespace pbl {
@@ -119,27 +121,45 @@ struct Tile {
     int nt;         // tile of output channels
 };
 
+// inclusive prefix sum over the wave's 64 lanes
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of rows 0 and 2 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {  // in lane 63
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return v;
+}
+
 template <int BM, int BAND>
 __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
     const int lane = threadIdx.x & 63;
-    auto rows_of = [&](int g, int &lo, int &hi) {
-        lo = 0;
-        hi = a.m;
-        if (a.offsets) {
-            lo = min(max(a.offsets[g], 0), a.m);
-            hi = min(max(a.offsets[g + 1], 0), a.m);
-            hi = max(lo, hi);
+    // group g0 + lane: its rows, and how many tiles the groups g0 .. g0 + lane have
+    int lo = 0, hi = 0, c = 0, inc = 0;
+    auto look = [&](int g0) {
+        lo = hi = 0;
+        if (g0 + lane < a.groups) {
+            lo = min(max(a.offsets[g0 + lane], 0), a.m);
+            hi = max(lo, min(a.offsets[g0 + lane + 1], a.m));
         }
+        c = (hi - lo + BM - 1) / BM;
+        inc = wave_prefix(c);
     };
     long m_tiles = 0;
     if (a.offsets) {
         for (int g0 = 0; g0 < a.groups; g0 += 64) {
-            int lo = 0, hi = 0;
-            if (g0 + lane < a.groups) rows_of(g0 + lane, lo, hi);
-            int c = (hi - lo + BM - 1) / BM;
-#pragma unroll
-            for (int s = 32; s; s >>= 1) c += __shfl_xor(c, s);
-            m_tiles += c;
+            look(g0);
+            m_tiles += __builtin_amdgcn_readlane(inc, 63);
         }
     } else m_tiles = (a.m + BM - 1) / BM;
     Tile t = {0, 0, 0, 0};
@@ -158,28 +178,16 @@ __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
         return t;
     }
     for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        int lo = 0, hi = 0;
-        if (g0 + lane < a.groups) rows_of(g0 + lane, lo, hi);
-        const int c = (hi - lo + BM - 1) / BM;
-        int inc = c;
-#pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int o = __shfl_up(inc, s);
-            if (lane >= s) inc += o;
-        }
+        if (a.groups > 64) look(g0);
         const uint64_t past = __ballot(inc > mt);
         if (past) {
-            const int l = __ffsll((unsigned long long)past) - 1;
+            const int l = __builtin_ctzll(past);
             t.g = g0 + l;
-            const int first = __shfl(inc - c, l);
-            t.r0 = __shfl(lo, l) + (mt - first) * BM;
-            t.r1 = min(t.r0 + BM, __shfl(hi, l));
-            t.g = __builtin_amdgcn_readfirstlane(t.g);
-            t.r0 = __builtin_amdgcn_readfirstlane(t.r0);
-            t.r1 = __builtin_amdgcn_readfirstlane(t.r1);
+            t.r0 = __builtin_amdgcn_readlane(lo, l) + (mt - __builtin_amdgcn_readlane(inc - c, l)) * BM;
+            t.r1 = min(t.r0 + BM, __builtin_amdgcn_readlane(hi, l));
             return t;
         }
-        mt -= __shfl(inc, 63);
+        mt -= __builtin_amdgcn_readlane(inc, 63);
     }
     return t;
 }
@@ -190,8 +198,14 @@ __device__ __forceinline__ float act_f(float v, int act) {
     if (act == PB_ACT_TANH) return tanhf(v);
     return v;
 }
-__device__ __forceinline__ uint16_t bits_bf16(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
-__device__ __forceinline__ uint16_t bits_f16(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// two values rounded to the nearest bf16 / f16 (halves to even), packed
+__device__ __forceinline__ uint32_t pack2(float x, float y, int type) {
+    const f32x2 v = {x, y};
+    return type == BF16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2)) : __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
 
 // W consecutive channels [c0, ..) of y row yr
 template <int W>
@@ -211,23 +225,16 @@ __device__ __forceinline__ void store_row(const LinearArgs &a, int yr, int c0, c
         }
     } else {
         uint16_t *p = reinterpret_cast<uint16_t *>(row) + c0;
-        uint16_t h[W];
+        uint32_t h[W / 2];
 #pragma unroll
-        for (int i = 0; i < W; ++i) h[i] = a.y_type == BF16 ? bits_bf16(v[i]) : bits_f16(v[i]);
+        for (int i = 0; i < W / 2; ++i) h[i] = pack2(v[2 * i], v[2 * i + 1], a.y_type);
         if (whole) {
-            if constexpr (W == 8) {
-                u32x4 q;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) q[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-                *reinterpret_cast<u32x4 *>(p) = q;
-            } else {
-                const u32x2 q = {h[0] | ((uint32_t)h[1] << 16), h[2] | ((uint32_t)h[3] << 16)};
-                *reinterpret_cast<u32x2 *>(p) = q;
-            }
+            if constexpr (W == 8) *reinterpret_cast<u32x4 *>(p) = u32x4{h[0], h[1], h[2], h[3]};
+            else *reinterpret_cast<u32x2 *>(p) = u32x2{h[0], h[1]};
         } else {
 #pragma unroll
             for (int i = 0; i < W; ++i)
-                if (c0 + i < a.n) p[i] = h[i];
+                if (c0 + i < a.n) p[i] = (uint16_t)(h[i / 2] >> (16 * (i & 1)));
         }
     }
 }
@@ -244,15 +251,27 @@ template <int T, int W> struct Chan {
             bias[i] = a.bias && in ? a.bias[at] : 0.0f;
         }
     }
+    // PLAIN: no activation, whole vectors of a known type YT -- what the large products mostly are, without a branch per row
+    template <bool PLAIN = false, int YT = 0>
     __device__ __forceinline__ void finish(const LinearArgs &a, const typename Acc<T>::e (&s)[W], float row_scale, int yr, int c0) const {
         float v[W];
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             v[i] = (float)s[i];
             if constexpr (T == I8) v[i] = v[i] * row_scale * scale[i];
-            v[i] = act_f(v[i] + bias[i], a.act);
+            v[i] += bias[i];
+            if constexpr (!PLAIN) v[i] = act_f(v[i], a.act);
         }
-        store_row<W>(a, yr, c0, v);
+        if constexpr (!PLAIN) store_row<W>(a, yr, c0, v);
+        else if constexpr (YT == F32) {
+            float *p = reinterpret_cast<float *>(a.y + (long)yr * a.ldy) + c0;
+#pragma unroll
+            for (int i = 0; i < W; i += 4) *reinterpret_cast<f32x4 *>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+        } else {
+            static_assert(W == 8, "");
+            *reinterpret_cast<u32x4 *>(reinterpret_cast<uint16_t *>(a.y + (long)yr * a.ldy) + c0) =
+                u32x4{pack2(v[0], v[1], YT), pack2(v[2], v[3], YT), pack2(v[4], v[5], YT), pack2(v[6], v[7], YT)};
+        }
     }
 };
 
@@ -284,19 +303,18 @@ __device__ __forceinline__ void rows_to_lds(const LinearArgs &a, const Tile &t, 
 
 // A wave's sums -> y, 32 rows x WN channels at a time: they go to LDS as the matrix instruction left them (4 consecutive channels per
 // lane) and come back as 8 consecutive channels per lane, whole rows by consecutive lanes.  s_mem: 32 (WN + 4) sums for each wave.
-template <int T, int MT, int NT, int WN>
-__device__ __forceinline__ void store_tile(const LinearArgs &a, int g, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem, const int *yrows,
-                                           const float *scales, int wave, int lane, int c_wave) {
+template <int T, int MT, int NT, int WN, bool PLAIN, int YT>
+__device__ __forceinline__ void store_rows(const LinearArgs &a, const Chan<T, 8> &ch, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem,
+                                           const int *yrows, const float *scales, int wave, int lane, int c0, int valid) {
     typedef typename Acc<T>::e E;
     typedef typename Acc<T>::q4 Q;
     constexpr int PITCH = WN + 4;
     E *img = reinterpret_cast<E *>(s_mem) + wave * 32 * PITCH;
     constexpr int LPR = WN / 8, RPI = 64 / LPR;  // lanes per row, rows per instruction
-    const int li = lane & 31, hi = lane >> 5;
-    const int c8 = (lane % LPR) * 8, c0 = c_wave + c8;
-    const Chan<T, 8> ch(a, g, c0);
+    const int li = lane & 31, hi = lane >> 5, c8 = (lane % LPR) * 8;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
+        if (i * 32 >= valid) break;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -306,14 +324,25 @@ __device__ __forceinline__ void store_tile(const LinearArgs &a, int g, const typ
             }
         __builtin_amdgcn_wave_barrier();  // one wave's LDS accesses are in order
 #pragma unroll
-        for (int r = lane / LPR; r < 32; r += RPI) {
-            const int yr = yrows[i * 32 + r];
-            const Q lo = *reinterpret_cast<const Q *>(img + r * PITCH + c8), up = *reinterpret_cast<const Q *>(img + r * PITCH + c8 + 4);
+        for (int r = 0; r < 32; r += RPI) {
+            const int at = r + lane / LPR, yr = yrows[i * 32 + at];
+            const Q lo = *reinterpret_cast<const Q *>(img + at * PITCH + c8), up = *reinterpret_cast<const Q *>(img + at * PITCH + c8 + 4);
             const E s[8] = {lo[0], lo[1], lo[2], lo[3], up[0], up[1], up[2], up[3]};
-            if (yr >= 0) ch.finish(a, s, T == I8 ? scales[i * 32 + r] : 1.0f, yr, c0);
+            if (yr >= 0) ch.template finish<PLAIN, YT>(a, s, T == I8 ? scales[i * 32 + at] : 1.0f, yr, c0);
         }
         __builtin_amdgcn_wave_barrier();
     }
+}
+template <int T, int MT, int NT, int WN>
+__device__ __forceinline__ void store_tile(const LinearArgs &a, int g, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem, const int *yrows,
+                                           const float *scales, int wave, int lane, int c_wave, int valid) {
+    const int c0 = c_wave + (lane % (WN / 8)) * 8;
+    const Chan<T, 8> ch(a, g, c0);
+    const bool plain = a.act == PB_ACT_NONE && a.y_vec && c_wave + WN <= a.n;  // of the whole wave
+    if (plain && a.y_type == BF16) store_rows<T, MT, NT, WN, true, BF16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
+    else if (plain && a.y_type == F16) store_rows<T, MT, NT, WN, true, F16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
+    else if (plain) store_rows<T, MT, NT, WN, true, F32>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
+    else store_rows<T, MT, NT, WN, false, F32>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
 }
 
 // ---- k_linear_tile: a tile of BM rows x BN channels per workgroup, K in steps of 128 bytes through LDS ------------------------------------
@@ -369,31 +398,35 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
         }
     };
     u32x4 regs[DMA ? 1 : J];
-    auto load_regs = [&](int i) {
+    auto load_regs = [&](int i, u32x4 (&to)[DMA ? 1 : J]) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) regs[DMA ? 0 : j] = load16<false>(pp[j] + (long)i * 128);
+        for (int j = 0; j < J; ++j) to[DMA ? 0 : j] = load16<false>(pp[j] + (long)i * 128);
     };
-    auto put_regs = [&](int i) {
+    auto put_regs = [&](int i, const u32x4 (&from)[DMA ? 1 : J]) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = regs[DMA ? 0 : j];
+        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = from[DMA ? 0 : j];
     };
     const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 31, hi = lane >> 5;
     typename Acc<T>::q16 acc[NT][MT] = {};
     const uint8_t *sa = s_mem + (wm + li) * 128, *sb = s_mem + (BM + wn + li) * 128;
     u32x4 fa[NF][MT], fb[NF][NT];
-    auto read = [&](int i, int ks, int to) {
+    // MV: the 32-row pieces of this wave that hold rows -- a group's last tile is seldom full, and matrix instructions on nothing
+    // would cost as much as others
+    auto read = [&](auto MV, int i, int ks, int to) {
         const int c = (i & (NST - 1)) * STAGE + ((ks * 2 + hi) ^ ((li >> 1) & 7)) * 16;
+        if constexpr (MV.value > 0) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) fb[to][j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
+            for (int j = 0; j < NT; ++j) fb[to][j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
+        }
 #pragma unroll
-        for (int m = 0; m < MT; ++m) fa[to][m] = *reinterpret_cast<const u32x4 *>(sa + m * 4096 + c);
+        for (int m = 0; m < MV.value; ++m) fa[to][m] = *reinterpret_cast<const u32x4 *>(sa + m * 4096 + c);
     };
     // a piece; `send`: the loads of step i among its matrix instructions
-    auto multiply = [&](int from, bool send, int i) {
+    auto multiply = [&](auto MV, int from, bool send, int i) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m) mma32<T>(acc[j][m], fb[from][j], fa[from][m]);
+            for (int m = 0; m < MV.value; ++m) mma32<T>(acc[j][m], fb[from][j], fa[from][m]);
             if constexpr (DMA) {
                 if (send) {
 #pragma unroll
@@ -410,16 +443,21 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
         else if (NST > 2 && younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
-    for (int i = 0; i < NST; ++i) {
+    // the first steps: all stages, or (FLAT through registers) the first step, with the second one's loads on their way
+    constexpr int AHEAD = FLAT && !DMA ? 1 : NST;
+    for (int i = 0; i < AHEAD; ++i) {
         if (i < full) {
             if constexpr (DMA) {
 #pragma unroll
                 for (int j = 0; j < J; ++j) dma(i, j);
             } else {
-                load_regs(i);
-                put_regs(i);
+                load_regs(i, regs);
+                put_regs(i, regs);
             }
         } else if (i < steps) copy_tail(i);
+    }
+    if constexpr (FLAT && !DMA) {
+        if (1 < full) load_regs(1, regs);
     }
     auto barrier = [&] {  // this wave's LDS reads have come back, its LDS writes are done
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -427,50 +465,68 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
         asm volatile("s_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    if constexpr (FLAT) {
-        for (int i = 0; i < steps; ++i) {
-            landed(i);
-            barrier();  // step i is in LDS, everyone has read step i - 1
-            const int next = i - 1 + NST;
-            const bool more = i > 0 && next < full;
-            if (more) {
-                if constexpr (DMA) {
+    auto walk = [&](auto MV) {
+        if constexpr (FLAT && DMA) {
+            for (int i = 0; i < steps; ++i) {
+                landed(i);
+                barrier();  // step i is in LDS, everyone has read step i - 1
+                const int next = i - 1 + NST;
+                if (i > 0 && next < full) {
 #pragma unroll
                     for (int j = 0; j < J; ++j) dma(next, j);
-                } else load_regs(next);
-            } else if (i > 0 && next == full && full < steps) copy_tail(full);
+                } else if (i > 0 && next == full && full < steps) copy_tail(full);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) read(i, ks, ks);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int ks = 0; ks < 4; ++ks) read(MV, i, ks, ks);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) multiply(ks, false, 0);
-            if constexpr (!DMA) {
-                if (more) put_regs(next);
+                for (int ks = 0; ks < 4; ++ks) multiply(MV, ks, false, 0);
+            }
+        } else if constexpr (FLAT) {
+            // step i + 2's registers are loaded while step i is multiplied, step i + 1's go to LDS behind it
+            auto half = [&](int i, u32x4 (&now)[DMA ? 1 : J], u32x4 (&later)[DMA ? 1 : J]) {
+                barrier();  // step i is in LDS, everyone has read step i - 1
+                if (i + 2 < full) load_regs(i + 2, later);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) read(MV, i, ks, ks);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) multiply(MV, ks, false, 0);
+                if (i + 1 < full) put_regs(i + 1, now);
+                else if (i + 1 == full && full < steps) copy_tail(full);
+            };
+            u32x4 other[DMA ? 1 : J];
+            for (int i = 0; i < steps; i += 2) {
+                half(i, regs, other);
+                if (i + 1 < steps) half(i + 1, other, regs);
+            }
+        } else {
+            landed(0);
+            barrier();
+            if (steps > 0) read(MV, 0, 0, 0);
+            for (int i = 0; i < steps; ++i) {
+                const bool more = !DMA && i > 0 && i + NST - 1 < full;
+                if (more) load_regs(i + NST - 1, regs);
+                read(MV, i, 1, 1);
+                multiply(MV, 0, false, 0);
+                read(MV, i, 2, 0);
+                multiply(MV, 1, false, 0);
+                read(MV, i, 3, 1);
+                multiply(MV, 0, false, 0);
+                if (more) put_regs(i + NST - 1, regs);
+                landed(i + 1);
+                barrier();  // the last piece's fragments are in registers everywhere, step i + 1 is in LDS
+                if (i + NST == full && full < steps) copy_tail(full);
+                if (i + 1 < steps) read(MV, i + 1, 0, 0);
+                multiply(MV, 1, DMA && i + NST < full, i + NST);
             }
         }
-    } else {
-        landed(0);
-        barrier();
-        if (steps > 0) read(0, 0, 0);
-        for (int i = 0; i < steps; ++i) {
-            const bool more = !DMA && i > 0 && i + NST - 1 < full;
-            if (more) load_regs(i + NST - 1);
-            read(i, 1, 1);
-            multiply(0, false, 0);
-            read(i, 2, 0);
-            multiply(1, false, 0);
-            read(i, 3, 1);
-            multiply(0, false, 0);
-            if (more) put_regs(i + NST - 1);
-            landed(i + 1);
-            barrier();  // the last piece's fragments are in registers everywhere, step i + 1 is in LDS
-            if (i + NST == full && full < steps) copy_tail(full);
-            if (i + 1 < steps) read(i + 1, 0, 0);
-            multiply(1, DMA && i + NST < full, i + NST);
-        }
-    }
+    };
+    const int valid = t.r1 - t.r0 - wm;  // rows of this wave's part
+    if (valid <= 0) walk(std::integral_constant<int, 0>{});
+    else if (MT > 1 && valid <= WM / 2) walk(std::integral_constant<int, (MT > 1 ? MT / 2 : MT)>{});
+    else walk(std::integral_constant<int, MT>{});
     __syncthreads();  // the stages become the waves' epilogue images
-    store_tile<T, MT, NT, WN>(a, t.g, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn);
+    store_tile<T, MT, NT, WN>(a, t.g, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn, valid);
 }
 
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
@@ -490,27 +546,28 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     const int c_base = t.nt * BN;
     const uint8_t *px[MT], *pw[NT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) px[i] = a.x + (long)max(x_row_of(a, min(t.r0 + i * 16 + li, t.r1 - 1)), 0) * a.ldx;
+    for (int i = 0; i < MT; ++i) px[i] = a.x + (long)max(x_row_of(a, min(t.r0 + i * 16 + li, t.r1 - 1)), 0) * a.ldx + kq;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) pw[j] = a.w + ((long)t.g * a.n + min(c_base + j * 16 + li, a.n - 1)) * a.ldw;
+    for (int j = 0; j < NT; ++j) pw[j] = a.w + ((long)t.g * a.n + min(c_base + j * 16 + li, a.n - 1)) * a.ldw + kq;
     Q acc[NT][MT] = {};
-    for (long kb = (long)wave * 64 * U; kb < a.kb; kb += 64 * U * NW) {
+    const int kb1 = (int)a.kb;
+    for (int kb = wave * 64 * U; kb < kb1; kb += 64 * U * NW) {
         u32x4 fw[U][NT], fx[U][MT];
-        if (kb + 64 * U <= a.kb) {
+        if (kb + 64 * U <= kb1) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16<ALIGNED>(pw[j] + kb + u * 64 + kq);
+                for (int j = 0; j < NT; ++j) fw[u][j] = load16<ALIGNED>(pw[j] + kb + u * 64);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16<ALIGNED>(px[i] + kb + u * 64 + kq);
+                for (int i = 0; i < MT; ++i) fx[u][i] = load16<ALIGNED>(px[i] + kb + u * 64);
             }
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail<ALIGNED>(pw[j], kb + u * 64 + kq, a.kb);
+                for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail<ALIGNED>(pw[j] - kq, kb + u * 64 + kq, kb1);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail<ALIGNED>(px[i], kb + u * 64 + kq, a.kb);
+                for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail<ALIGNED>(px[i] - kq, kb + u * 64 + kq, kb1);
             }
         }
 #pragma unroll
@@ -544,17 +601,46 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 }
 
 // ---- k_quantize_rows ------------------------------------------------------------------------------------------------------------------------
-// scale = max(max |x| / 127, 2^-126); code = x / scale to the nearest whole number, halves to the even one.  The code is decided
-// exactly without a division per value: r = rint(x * (1 / scale)) is off by at most one, and x - r * scale, which one fused
-// multiply-add gives exactly wherever it is near scale / 2, says on which side of the half x lies.  A row with an infinity or a
-// NaN gets scale = NaN and codes 0, so that what is computed from it shows.
-__device__ __forceinline__ int code_of(float x, float inv, float scale, float half) {
-    float r = rintf(x * inv);
+// scale = max(max |x| / 127, 2^-126); code = x / scale to the nearest whole number, halves to the even one.  Without a division per
+// value, and exactly: x * (1 / scale) + 1.5 * 2^23, one fused multiply-add, is the whole number in the low bits (1 / scale is off by
+// half a unit in the last place, the quotient by less than 7.7e-6).  Only where it lies within 1e-5 of a half -- one value in 50 000 -- the
+// remainder x - r * scale decides, which a fused multiply-add gives exactly near scale / 2.  A row with an infinity or a NaN gets
+// scale = NaN and codes 0, so that what is computed from it shows.
+constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
+__device__ __forceinline__ uint32_t code_exact(float x, float inv, float scale, float half) {
+    float r = rintf(x * inv);  // off by one at most
     const float d = __builtin_fmaf(-r, scale, x), ad = fabsf(d);
-    const float up = d > 0.0f ? 1.0f : -1.0f;
     const bool odd = ((int)r & 1) != 0;
-    if (ad > half || (ad == half && odd)) r += up;
-    return (int)r;
+    if (ad > half || (ad == half && odd)) r += d > 0.0f ? 1.0f : -1.0f;
+    return (uint32_t)(int)r;
+}
+// V codes, packed four to a word
+template <int V>
+__device__ __forceinline__ void codes_of(const float (&x)[V], float inv, float scale, float half, uint32_t (&word)[V / 4]) {
+    uint32_t q[V];
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float r = __builtin_fmaf(x[i], inv, MAGIC);
+        q[i] = __float_as_uint(r);
+        far = fmaxf(far, fabsf(__builtin_fmaf(x[i], inv, MAGIC - r)));
+    }
+    if (far > 0.49999f) {
+#pragma unroll 1
+        for (int i = 0; i < V; ++i) {
+            float v = x[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) v = i == j ? x[j] : v;
+            const uint32_t c = code_exact(v, inv, scale, half);
+#pragma unroll
+            for (int j = 0; j < V; ++j) q[j] = i == j ? c : q[j];
+        }
+    }
+#pragma unroll
+    for (int w = 0; w < V / 4; ++w) {
+        const uint32_t lo = __builtin_amdgcn_perm(q[4 * w + 1], q[4 * w], 0x0c0c0400u), up = __builtin_amdgcn_perm(q[4 * w + 3], q[4 * w + 2], 0x0c0c0400u);
+        word[w] = lo | (up << 16);
+    }
 }
 
 template <int T> __device__ __forceinline__ float elem(const uint8_t *row, long i) {
@@ -563,21 +649,23 @@ template <int T> __device__ __forceinline__ float elem(const uint8_t *row, long 
     else return (float)reinterpret_cast<const _Float16 *>(row)[i];
 }
 
-// A workgroup of NTHR threads per row, V values per thread and turn; rows of up to NTHR * V * TURNS values stay in registers between
-// the maximum and the codes, longer ones are read a second time.  VEC: 16-byte loads (rows start on 16 bytes, codes on V).
+// NTHR threads per row (a wave or a workgroup of four), V values per thread and turn; rows of up to NTHR * V * TURNS values stay in
+// registers between the maximum and the codes, longer ones are read a second time.  VEC: 16-byte loads (rows start on 16 bytes,
+// codes on V).
 template <int T, int NTHR, int TURNS, bool VEC>
-__global__ __launch_bounds__(NTHR) void k_quantize_rows(const uint8_t *__restrict__ x, long m, int k, long ldx, int8_t *__restrict__ codes, long ldc,
-                                                        float *__restrict__ scale) {
-    constexpr int V = T == F32 ? 4 : 8;
-    __shared__ uint32_t s_max[NTHR / 64];
-    const int tid = threadIdx.x;
-    const long row = blockIdx.x;
-    const uint8_t *px = x + row * ldx;
-    int8_t *pc = codes + row * ldc;
+__global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict__ x, int m, int k, long ldx, int8_t *__restrict__ codes, long ldc,
+                                                       float *__restrict__ scale) {
+    constexpr int V = T == F32 ? 4 : 8, RPB = 256 / NTHR;
+    __shared__ uint32_t s_max[4];
+    const int tid = threadIdx.x % NTHR;
+    const int row = blockIdx.x * RPB + (RPB > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0);
+    if (row >= m) return;
+    const uint8_t *px = x + (long)row * ldx;
+    int8_t *pc = codes + (long)row * ldc;
     const uint32_t INF = 0x7f800000u;
-    auto load = [&](long c, float (&v)[V]) {
+    auto load = [&](int c, float (&v)[V]) {
         if (VEC && c + V <= k) {
-            const u32x4 q = *reinterpret_cast<const u32x4 *>(px + c * type_bytes(T));
+            const u32x4 q = *reinterpret_cast<const u32x4 *>(px + (long)c * type_bytes(T));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if constexpr (T == F32) v[i] = __uint_as_float(q[i]);
@@ -592,44 +680,45 @@ __global__ __launch_bounds__(NTHR) void k_quantize_rows(const uint8_t *__restric
     float v[TURNS][V];
     uint32_t top = 0;  // |x| as bits: the order of non-negative floats, infinities and NaN above all of them
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {
-        load(((long)t * NTHR + tid) * V, v[t]);
+    for (int t = 0; t < TURNS; ++t) load((t * NTHR + tid) * V, v[t]);
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t)
 #pragma unroll
         for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(v[t][i]) & 0x7fffffffu);
-    }
-    for (long c = ((long)TURNS * NTHR + tid) * V; c < k; c += (long)NTHR * V) {
+    for (int c = (TURNS * NTHR + tid) * V; c < k; c += NTHR * V) {
         float u[V];
         load(c, u);
 #pragma unroll
         for (int i = 0; i < V; ++i) top = max(top, __float_as_uint(u[i]) & 0x7fffffffu);
     }
-#pragma unroll
-    for (int s = 32; s; s >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, s));
+    top = (uint32_t)__builtin_amdgcn_readlane((int)wave_max(top), 63);
     if constexpr (NTHR > 64) {
         if ((tid & 63) == 0) s_max[tid >> 6] = top;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NTHR / 64; ++w) top = max(top, s_max[w]);
+        top = max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3]));
     }
     const bool bad = top >= INF;
-    const float sc = bad ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(top) / 127.0f, 1.17549435e-38f);
-    if (tid == 0) scale[row] = sc;
-    const float inv = 1.0f / sc, half = 0.5f * sc;
-    auto put = [&](long c, const float (&u)[V]) {
+    const float sc = fmaxf(__uint_as_float(top) / 127.0f, 1.17549435e-38f);
+    if (tid == 0) scale[row] = bad ? __uint_as_float(0x7fc00000u) : sc;
+    const float inv = bad ? 0.0f : 1.0f / sc, half = 0.5f * sc;
+    auto put = [&](int c, float (&u)[V]) {
         if (c >= k) return;
-        int8_t q[V];
+        if (bad) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) q[i] = bad ? (int8_t)0 : (int8_t)code_of(u[i], inv, sc, half);
-        if (VEC && c + V <= k) __builtin_memcpy(__builtin_assume_aligned(pc + c, V), q, V);
+            for (int i = 0; i < V; ++i) u[i] = 0.0f;
+        }
+        uint32_t w[V / 4];
+        codes_of<V>(u, inv, sc, half, w);
+        if (VEC && c + V <= k) __builtin_memcpy(__builtin_assume_aligned(pc + c, V), w, V);
         else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (c + i < k) pc[c + i] = q[i];
+                if (c + i < k) pc[c + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
         }
     };
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) put(((long)t * NTHR + tid) * V, v[t]);
-    for (long c = ((long)TURNS * NTHR + tid) * V; c < k; c += (long)NTHR * V) {
+    for (int t = 0; t < TURNS; ++t) put((t * NTHR + tid) * V, v[t]);
+    for (int c = (TURNS * NTHR + tid) * V; c < k; c += NTHR * V) {
         float u[V];
         load(c, u);
         put(c, u);
@@ -639,104 +728,125 @@ __global__ __launch_bounds__(NTHR) void k_quantize_rows(const uint8_t *__restric
 // ---- k_group_rows ---------------------------------------------------------------------------------------------------------------------------
 // Workgroup g < groups counts the rows of smaller groups (its offset) and lists its own rows in ascending order; workgroup `groups`
 // lists the rows without a group behind all others.  Every workgroup reads the whole array (it sits in L2) instead of meeting the
-// others: no scratch memory, no atomics, one launch, one possible result.  A wave owns a contiguous segment, a lane four
-// consecutive rows of each 256, and remembers its matches as bits, so that up to 131 072 rows are read once.
-constexpr int GR_WAVES = 16, GR_TURNS = 32, GR_CHUNK = GR_WAVES * GR_TURNS * 256;
+// others: no scratch memory, no atomics, one launch, one possible result.  A first walk, four consecutive rows per lane, turns each
+// comparison into a lane mask: the counts come from the scalar unit's bit counts, the masks of matching rows go to LDS -- four
+// vector instructions for 64 rows, which is what bounds it (131072 rows, 256 groups: 27 us with a bit per lane put together by vector
+// instructions).  Then every thread takes a contiguous run of words of 32 rows, learns by a prefix sum over the bit counts where its
+// rows go, and writes them.  Rows beyond one LDS map's 8192 per wave are walked a second time, map by map.
+// As unsigned numbers, rows of no group are >= groups: a row is before group g if it is < g.
+// v with the wave-uniform `value` in one lane: v_writelane_b32 as the compiler's intrinsic, which has no builtin of its own (as inline
+// asm the compiler leaves out the two wait states between the comparison that writes the scalar register and this read of it)
+extern "C" __device__ __attribute__((const)) int pb_writelane(int value, int lane, int v) __asm("llvm.amdgcn.writelane.i32");
 
-__global__ __launch_bounds__(64 * GR_WAVES) void k_group_rows(const int32_t *__restrict__ group, int m, int groups, int vec, int32_t *__restrict__ offsets,
+template <int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 8) void k_group_rows(const int32_t *__restrict__ group, int m, int groups, int vec, int32_t *__restrict__ offsets,
                                                               int32_t *__restrict__ order) {
-    __shared__ int s_lt[GR_WAVES], s_eq[GR_WAVES];
-    const int g = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int chunks = (m + GR_CHUNK - 1) / GR_CHUNK;  // m = 0: none
-    int seg = 0;
-    uint32_t bits[GR_TURNS / 8];  // 4 bits for each turn
-    int lt = 0, eq = 0;
-    auto look = [&](long at, int n, uint32_t &eq4, int &lt4) {  // rows [at, at + 4) of the n below the segment's end
-        int id[4];
-        if (vec && at + 4 <= n) {
-            const i32x4 q = *reinterpret_cast<const i32x4 *>(group + at);
-            id[0] = q.x; id[1] = q.y; id[2] = q.z; id[3] = q.w;
-        } else {
+    constexpr int NTHR = 64 * WAVES, CHUNK = WAVES * 8192;
+    __shared__ uint32_t s_mask[CHUNK / 32];  // per 256 rows eight words: rows 4 l + i of lane l at bit l of pair i
+    __shared__ int s_lt[WAVES], s_eq[WAVES];
+    const unsigned g = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunks = (int)(((long)m + CHUNK - 1) / CHUNK);  // m = 0: none
+    int lt = 0;  // rows before this group, of this wave's 256s
+    auto walk = [&](auto LAST, int c) {  // a wave takes every WAVES-th 256 rows
+        const int32_t *p = group + (long)c * CHUNK;
+        const int n = (int)min((long)CHUNK, (long)m - (long)c * CHUNK);
+        int turn = wave;
+        if (vec) {
+            for (; (turn + 7 * WAVES + 1) * 256 <= n; turn += 8 * WAVES) {
+                i32x4 q[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) id[i] = at + i < n ? group[at + i] : -2;
-        }
-        eq4 = 0;
-        lt4 = 0;
+                for (int j = 0; j < 8; ++j) q[j] = *reinterpret_cast<const i32x4 *>(p + (turn + j * WAVES) * 256 + lane * 4);
+                int words = 0;  // lane 8 j + 2 i + h: half h of turn j's mask i
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool in = at + i < n, has = (unsigned)id[i] < (unsigned)groups;
-            const int key = has ? id[i] : groups;
-            eq4 |= (in && key == g ? 1u : 0u) << i;
-            lt4 += in && key < g ? 1 : 0;
-        }
-    };
-    auto scan_chunk = [&](int c) {  // fills bits and eq of this wave's segment of chunk c, adds to lt
-        const long base = (long)c * GR_CHUNK;
-        const int n = (int)min((long)GR_CHUNK, (long)m - base);
-        seg = ((n + GR_WAVES - 1) / GR_WAVES + 255) & ~255;
-        eq = 0;
+                for (int j = 0; j < 8; ++j) {
 #pragma unroll
-        for (int w = 0; w < GR_TURNS / 8; ++w) {
-            bits[w] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int t = w * 8 + j;
-                if (t * 256 >= seg) break;
-                const long at = base + (long)wave * seg + t * 256 + lane * 4;
-                uint32_t e4;
-                int l4;
-                look(at, (int)min((long)m, base + n), e4, l4);
-                bits[w] |= e4 << (4 * j);
-                lt += l4;
-            }
-            eq += __builtin_popcount(bits[w]);
-        }
-    };
-    auto wave_sum = [&](int v) {
-#pragma unroll
-        for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
-        return v;
-    };
-    for (int c = 0; c < chunks; ++c) scan_chunk(c);
-    const int wl = wave_sum(lt);
-    if (lane == 0) s_lt[wave] = wl;
-    __syncthreads();
-    int first = 0;
-#pragma unroll
-    for (int w = 0; w < GR_WAVES; ++w) first += s_lt[w];
-    if (threadIdx.x == 0) offsets[g] = first;  // workgroup `groups`: the number of rows that have a group
-    for (int c = 0; c < chunks; ++c) {
-        if (chunks > 1) scan_chunk(c);
-        const int we = wave_sum(eq);
-        __syncthreads();  // the last chunk's counts have been read
-        if (lane == 0) s_eq[wave] = we;
-        __syncthreads();
-        int at = first;
-#pragma unroll
-        for (int w = 0; w < GR_WAVES; ++w) {
-            if (w < wave) at += s_eq[w];
-            first += s_eq[w];
-        }
-        const long base = (long)c * GR_CHUNK + (long)wave * seg;
-#pragma unroll
-        for (int w = 0; w < GR_TURNS / 8; ++w) {
-            if (__ballot(bits[w] != 0) == 0) continue;
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t e4 = (bits[w] >> (4 * j)) & 15u;
-                int before = 0, all = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint64_t b = __ballot((e4 >> i) & 1u);
-                    before += __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0u));
-                    all += __builtin_popcountll(b);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint64_t less = __ballot((unsigned)q[j][i] < g);
+                        const uint64_t own = LAST.value ? ~less : __ballot((unsigned)q[j][i] == g);
+                        lt += __builtin_popcountll(less);
+                        words = pb_writelane((int)(uint32_t)own, 8 * j + 2 * i, words);
+                        words = pb_writelane((int)(uint32_t)(own >> 32), 8 * j + 2 * i + 1, words);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // all 64 masks at once would not fit the scalar registers
                 }
+                s_mask[(turn + (lane >> 3) * WAVES) * 8 + (lane & 7)] = (uint32_t)words;
+            }
+        }
+#pragma unroll 1
+        for (; turn * 256 < n; turn += WAVES) {
+            const int at = turn * 256 + lane * 4;
+            i32x4 q = {-1, -1, -1, -1};
+            if (vec && at + 4 <= n) q = *reinterpret_cast<const i32x4 *>(p + at);
+            else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if ((e4 >> i) & 1u) order[at + before + __builtin_popcount(e4 & ((1u << i) - 1u))] = (int32_t)(base + (w * 8 + j) * 256 + lane * 4 + i);
-                at += all;
+                    if (at + i < n) q[i] = p[at + i];
             }
+            int words = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t less = __ballot((unsigned)q[i] < g);
+                const uint64_t own = LAST.value ? ~less & __ballot(at + i < n) : __ballot((unsigned)q[i] == g);
+                lt += __builtin_popcountll(less);
+                words = pb_writelane((int)(uint32_t)own, 2 * i, words);
+                words = pb_writelane((int)(uint32_t)(own >> 32), 2 * i + 1, words);
+            }
+            if (lane < 8) s_mask[turn * 8 + lane] = (uint32_t)words;
         }
-    }
+        return n;
+    };
+    auto run = [&](auto LAST) {
+        int n = 0;
+        for (int c = 0; c < chunks; ++c) n = walk(LAST, c);
+        if (lane == 0) s_lt[wave] = lt;
+        __syncthreads();
+        int first = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) first += s_lt[w];
+        if (tid == 0) offsets[g] = first;  // workgroup `groups`: the number of rows that have a group
+        for (int c = 0; c < chunks; ++c) {
+            if (chunks > 1) {
+                __syncthreads();  // the words and counts before these have been read
+                n = walk(LAST, c);
+                __syncthreads();
+            }
+            const int words = (n + 31) >> 5, each = (words + NTHR - 1) / NTHR;  // 1 .. 4 words for a thread
+            uint32_t b[4];
+            int count = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int w = tid * each + i;
+                b[i] = 0;
+                if (i < each && w < words) {  // word w: lanes 8 (w % 8) .. + 8 of turn w / 8, a bit of each of the four masks in turn
+                    const uint32_t *mask = s_mask + (w >> 3) * 8 + ((w >> 2) & 1);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t x = (mask[2 * k] >> (8 * (w & 3))) & 255u;
+                        x = (x | x << 12) & 0x000f000fu;
+                        x = (x | x << 6) & 0x03030303u;
+                        x = (x | x << 3) & 0x11111111u;
+                        b[i] |= x << k;
+                    }
+                }
+                count += __builtin_popcount(b[i]);
+            }
+            const int inc = wave_prefix(count);
+            if (lane == 63) s_eq[wave] = inc;
+            __syncthreads();
+            int to = first + inc - count;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if (w < wave) to += s_eq[w];
+                first += s_eq[w];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                for (uint32_t left = b[i]; left; left &= left - 1) order[to++] = c * CHUNK + (tid * each + i) * 32 + __builtin_ctz(left);
+        }
+    };
+    if (g == (unsigned)groups) run(std::true_type{});
+    else run(std::false_type{});
 }
 
 }  // namespace pbl
