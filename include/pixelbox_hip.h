@@ -275,6 +275,22 @@ int pb_embed_batch(pb_embedder *e, const uint8_t *rgb, uint32_t n, uint8_t *out_
 int pb_embed_batch_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, uint8_t *d_out_u8,
                           float *d_out_f32);
 
+/* The network up to its last layer: the pooled features (f32[n][1280], DEVICE, 16-byte aligned) that Linear(1280, D) + tanh make the
+ * hash of (resources/train.py:30-46), for layers of the caller's own (the linear layers below).  n <= max_batch; stream
+ * contract as pb_embed_batch_device. */
+int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, float *d_features);
+
+/* Several hash heads on one backbone: image i goes through the network once and through Linear(1280, d) + tanh of head d_head[i] (a
+ * collection, a user, a latent size of its own): forward -> pb_group_rows -> [pb_quantize_rows ->] pb_linear_grouped -> the u8
+ * quantiser of efficientnet.rs:39, all on the embedder's stream (contract as pb_embed_batch_device).  All pointers are DEVICE memory.
+ * type: PB_TYPE_F32 (d_w: f32[heads][d][1280]) or PB_TYPE_I8 (int8, with d_w_scale f32[heads][d]: pb_quantize_rows over the weights'
+ * rows); d_bias: f32[heads][d] or NULL; d_head: int[n].  d_out_u8: uint8[n][d], d_out_f32: f32[n][d], either may be NULL.  Images
+ * whose head is outside [0, heads) are left as they are in both.  The f32 product is summed in plain f32 (the embedder's own Linear
+ * sums bf16 pieces): with the blob's own weights as the only head the values agree with pb_embed_batch to the embedding's tolerance,
+ * not bit for bit.  An i8 head is off by the codes' rounding: half a code of 254 per feature and weight. */
+int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
+                          uint32_t heads, uint32_t d, const int *d_head, uint8_t *d_out_u8, float *d_out_f32);
+
 /* For PB_OPT_EMBED_ASYNC callers: PB_ERR_RANGE if a forward pass that has completed since the last check left the domain of the
  * fixed-point squeeze-excite sums (its outputs are not valid), PB_OK otherwise; clears the flag.  Call it after waiting for the
  * embedder's stream and before using the outputs of the batches queued since the last check: a queued pb_embed_batch_device call

@@ -76,6 +76,13 @@ struct pb_embedder {
     uint8_t *d_img = nullptr;
     float *buf_x[2] = {nullptr, nullptr};
     float *buf_e = nullptr, *buf_dw = nullptr, *buf_gate = nullptr, *buf_pool = nullptr;
+    // pb_embed_features_device / pb_embed_heads_device: where the running forward leaves its pooled features (it ends there, without
+    // the Linear); null: the ordinary forward.  hd_*: the heads' workspace, allocated at the first such call
+    float *feat_dst = nullptr;
+    float *hd_feat = nullptr, *hd_scale = nullptr, *hd_val = nullptr;
+    size_t hd_val_cap = 0;
+    int *hd_order = nullptr, *hd_offsets = nullptr;
+    int8_t *hd_codes = nullptr;
     long long *buf_part = nullptr;  // SE pooling partial sums, 2^-24 fixed point; buf_part[-1] holds the address of *h_range (se_range_check)
     unsigned *h_range = nullptr;    // pinned host word a kernel raises when an activation leaves the fixed-point domain (|x| >= 128)
     // pb_mlhash / pb_embed_batch with ONE image: input copy + the ~50 launches of the forward + output copies as one replayed hipGraph
@@ -1211,7 +1218,8 @@ int forward_device(pb_embedder *e, const uint8_t *d_rgb, int n, uint8_t *d_u8, f
     if (!e->ws2_ready && (rc = ws2_alloc(e))) return rc;
     const int n0 = (n + 1) / 2, n1 = n - n0;
     const uint8_t *rgb1 = d_rgb + (size_t)n0 * e->H * e->W * 3;
-    uint8_t *u81 = d_u8 + (size_t)n0 * e->D;
+    uint8_t *u81 = d_u8 ? d_u8 + (size_t)n0 * e->D : nullptr;
+    float *const feat0 = e->feat_dst, *const feat1 = feat0 ? feat0 + (size_t)n0 * 1280 : nullptr;
     float *f321 = d_f32 ? d_f32 + (size_t)n0 * e->D : nullptr;
     hipStream_t s0 = e->stream;
     // the second half starts where the caller's stream stands NOW (its input is there), not behind the first half
@@ -1220,11 +1228,18 @@ int forward_device(pb_embedder *e, const uint8_t *d_rgb, int n, uint8_t *d_u8, f
     if ((rc = forward_one(e, d_rgb, n0, d_u8, d_f32))) return rc;  // first half, on the caller's stream
     // a call that ran timing loops (the per-layer picks of this batch bucket) finishes one half after the other: a timing loop
     // must have the device to itself.  So does a split whose halves fall into different buckets.
-    if (e->tune_runs != before || tune_bucket(n0) != tune_bucket(n1)) return forward_one(e, rgb1, n1, u81, f321);
+    if (e->tune_runs != before || tune_bucket(n0) != tune_bucket(n1)) {
+        e->feat_dst = feat1;
+        rc = forward_one(e, rgb1, n1, u81, f321);
+        e->feat_dst = feat0;
+        return rc;
+    }
     PB_HIP(hipStreamWaitEvent(e->dual_stream, e->dual_e0, 0));
     ws_swap(e);
     e->stream = e->dual_stream;
+    e->feat_dst = feat1;
     rc = forward_one(e, rgb1, n1, u81, f321);
+    e->feat_dst = feat0;
     e->stream = s0;
     ws_swap(e);
     if (rc) {
@@ -1411,10 +1426,11 @@ int forward_rest(pb_embedder *e, const float *x_in, int n, size_t first, int H, 
     }
     const float *const xh = xr;
     const long M = (long)n * H * W;
+    float *const pool = e->feat_dst ? e->feat_dst : e->buf_pool;
     if (H * W == 16 && e->head.p3 && e->fc.p3 && !e->no_tail_fusion) {
         // P3 head + Linear with the same fused epilogues (pool in the head's accumulators; tanh + quantiser behind the Linear)
-        int rc = launch_p3_tuned(e, 1, p3_args(xh, M, e->head, nullptr, 16, nullptr, 1, e->buf_pool, 1.0f / 16.0f), e->head.wt2, "head + pool");
-        if (rc) return rc;
+        int rc = launch_p3_tuned(e, 1, p3_args(xh, M, e->head, nullptr, 16, nullptr, 1, pool, 1.0f / 16.0f), e->head.wt2, "head + pool");
+        if (rc || e->feat_dst) return rc;
         return launch_p3_tuned(e, 2, p3_args(e->buf_pool, n, e->fc, nullptr, 1, nullptr, 0, d_f32, 0.f, d_u8), e->fc.wt2, "linear + tanh + quantiser");
     }
     if (H * W == 16 && e->head.wt2 && e->fc.wt2 && !e->head.p3 && !e->fc.p3 && !e->no_tail_fusion) {
@@ -1424,8 +1440,8 @@ int forward_rest(pb_embedder *e, const float *x_in, int n, size_t first, int H, 
         const std::pair<const void *, long> key(e->head.wt2, tune_bucket(M));
         auto it = e->gemm_cfg.find(key);
         auto launch_head = [&](int nr, int nw) {
-            if (nw == 8) launch_gemm_t<false, 8, 1>(nr, e->stream, xh, M, e->head, nullptr, 16, nullptr, 1, e->buf_pool, 1.0f / 16.0f);
-            else launch_gemm_t<false, 4, 1>(nr, e->stream, xh, M, e->head, nullptr, 16, nullptr, 1, e->buf_pool, 1.0f / 16.0f);
+            if (nw == 8) launch_gemm_t<false, 8, 1>(nr, e->stream, xh, M, e->head, nullptr, 16, nullptr, 1, pool, 1.0f / 16.0f);
+            else launch_gemm_t<false, 4, 1>(nr, e->stream, xh, M, e->head, nullptr, 16, nullptr, 1, pool, 1.0f / 16.0f);
         };
         if (it == e->gemm_cfg.end()) {
             TuneTimer tt(e);
@@ -1458,6 +1474,7 @@ int forward_rest(pb_embedder *e, const float *x_in, int n, size_t first, int H, 
         }
         launch_head(it->second.second, it->second.first);
         PB_HIP(hipGetLastError());
+        if (e->feat_dst) return PB_OK;
         launch_gemm_t<false, 4, 2>(1, e->stream, e->buf_pool, n, e->fc, nullptr, 1, nullptr, 0, d_f32, 0.f, d_u8);
         PB_HIP(hipGetLastError());
         return PB_OK;
@@ -1465,8 +1482,9 @@ int forward_rest(pb_embedder *e, const float *x_in, int n, size_t first, int H, 
     int rc = launch_gemm(e, xh, M, e->head, nullptr, 1, nullptr, 1, e->buf_e);
     if (rc) return rc;
     hipLaunchKernelGGL(k_avgpool, dim3((1280 + 255) / 256, n), dim3(256), 0, e->stream, e->buf_e, H * W, 1280,
-                       1.0f / (float)(H * W), e->buf_pool);
+                       1.0f / (float)(H * W), pool);
     PB_HIP(hipGetLastError());
+    if (e->feat_dst) return PB_OK;
     if ((rc = launch_gemm(e, e->buf_pool, n, e->fc, nullptr, 1, nullptr, 0, e->buf_gate))) return rc;  // pre-tanh [n][D]
     {
         const long tot = (long)n * e->D;
@@ -1928,6 +1946,83 @@ int pb_embed_batch_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, uint
     // returned -- and consumed -- the flag of EARLIER batches: an error for a call whose own work was still in flight, and the batch
     // that raised it reported to whichever call came next).  The caller asks pb_embed_check_range after its stream wait.
     return PB_OK;
+}
+
+// the pooled features of n images on the embedder's stream
+static int forward_features(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, float *d_features) {
+    e->feat_dst = d_features;
+    const int rc = forward_device(e, d_rgb, (int)n, nullptr, nullptr);
+    e->feat_dst = nullptr;
+    return rc;
+}
+
+int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, float *d_features) {
+    PB_CHECK(e, PB_ERR_INVALID, "pb_embed_features_device: null embedder");
+    PB_CHECK(n <= e->max_batch, PB_ERR_INVALID, "pb_embed_features_device: n = %u > max_batch %u", n, e->max_batch);
+    PB_CHECK(n == 0 || (d_rgb && d_features), PB_ERR_INVALID, "pb_embed_features_device: null buffer");
+    PB_CHECK(((uintptr_t)d_features & 15) == 0, PB_ERR_INVALID, "pb_embed_features_device: d_features is not aligned to 16 bytes");
+    if (n == 0) return PB_OK;
+    std::lock_guard<std::mutex> lock(e->mu);
+    pb::DeviceGuard guard(e->device);
+    const int rc = forward_features(e, d_rgb, n, d_features);
+    if (rc || e->opt_async) return rc;
+    PB_HIP(hipStreamSynchronize(e->stream));
+    return range_status(e);
+}
+
+int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
+                          uint32_t heads, uint32_t d, const int *d_head, uint8_t *d_out_u8, float *d_out_f32) {
+    PB_CHECK(e, PB_ERR_INVALID, "pb_embed_heads_device: null embedder");
+    PB_CHECK(n <= e->max_batch, PB_ERR_INVALID, "pb_embed_heads_device: n = %u > max_batch %u", n, e->max_batch);
+    PB_CHECK(type == PB_TYPE_F32 || type == PB_TYPE_I8, PB_ERR_INVALID, "pb_embed_heads_device: weights are f32 or i8, not type %d", type);
+    PB_CHECK(heads >= 1 && heads <= PB_MAX_GROUPS, PB_ERR_INVALID, "pb_embed_heads_device: heads = %u (1 .. %u)", heads, PB_MAX_GROUPS);
+    PB_CHECK(d >= 1 && d <= (1u << 20), PB_ERR_INVALID, "pb_embed_heads_device: d = %u (1 .. 2^20)", d);
+    PB_CHECK(n == 0 || (d_rgb && d_w && d_head && (d_out_u8 || d_out_f32) && (type != PB_TYPE_I8 || d_w_scale)), PB_ERR_INVALID,
+             "pb_embed_heads_device: null buffer");
+    if (n == 0) return PB_OK;
+    std::lock_guard<std::mutex> lock(e->mu);
+    pb::DeviceGuard guard(e->device);
+    int rc;
+    const size_t B = e->max_batch;
+    if (!e->hd_feat) {
+        float *feat = nullptr;
+        if ((rc = dalloc(e, &e->hd_order, B)) || (rc = dalloc(e, &e->hd_offsets, (size_t)PB_MAX_GROUPS + 1)) || (rc = dalloc(e, &e->hd_codes, B * 1280)) ||
+            (rc = dalloc(e, &e->hd_scale, B)) || (rc = dalloc(e, &feat, B * 1280)))
+            return rc;
+        e->hd_feat = feat;
+    }
+    float *val = d_out_f32;
+    if (!val) {
+        if (e->hd_val_cap < B * d) {  // a wider head than any before: the smaller buffer goes once nothing queued uses it
+            if (e->hd_val) {
+                PB_HIP(hipStreamSynchronize(e->stream));
+                e->allocs.erase(std::find(e->allocs.begin(), e->allocs.end(), (void *)e->hd_val));
+                (void)hipFree(e->hd_val);
+                e->hd_val = nullptr;
+                e->hd_val_cap = 0;
+            }
+            if ((rc = dalloc(e, &e->hd_val, B * d))) return rc;
+            e->hd_val_cap = B * d;
+        }
+        val = e->hd_val;
+    }
+    if ((rc = forward_features(e, d_rgb, n, e->hd_feat))) return rc;
+    if ((rc = pb_group_rows(e->device, e->stream, d_head, n, heads, e->hd_offsets, e->hd_order))) return rc;
+    const void *x = e->hd_feat;
+    if (type == PB_TYPE_I8) {
+        if ((rc = pb_quantize_rows(e->device, e->stream, e->hd_feat, PB_TYPE_F32, n, 1280, 1280, e->hd_codes, 1280, e->hd_scale))) return rc;
+        x = e->hd_codes;
+    }
+    if ((rc = pb_linear_grouped(e->device, e->stream, type, x, n, 1280, e->hd_scale, d_w, 1280, d_w_scale, d_bias, e->hd_offsets, heads, e->hd_order,
+                                e->hd_order, PB_ACT_TANH, val, PB_TYPE_F32, n, d, n, d, 1280)))
+        return rc;
+    if (d_out_u8) {
+        hipLaunchKernelGGL(k_hash_rows, dim3((d + 255) / 256, n), dim3(256), 0, e->stream, val, d_head, (int)heads, (int)d, d_out_u8);
+        PB_HIP(hipGetLastError());
+    }
+    if (e->opt_async) return PB_OK;
+    PB_HIP(hipStreamSynchronize(e->stream));
+    return range_status(e);
 }
 
 int pb_embed_check_range(pb_embedder *e) {

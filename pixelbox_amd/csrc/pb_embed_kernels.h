@@ -2369,4 +2369,12 @@ __global__ void k_tanh_quant(const float *__restrict__ pre, long n, float *__res
     out_u8[i] = quantize_u8(y);
 }
 
+// the hash bytes (efficientnet.rs:39) of the images that have a head; the others' bytes are left as they are
+__global__ void k_hash_rows(const float *__restrict__ val, const int *__restrict__ head, int heads, int d, uint8_t *__restrict__ out_u8) {
+    const int j = blockIdx.x * blockDim.x + threadIdx.x;
+    const long row = blockIdx.y;
+    if (j >= d || (unsigned)head[row] >= (unsigned)heads) return;
+    out_u8[row * d + j] = quantize_u8(val[row * d + j]);
+}
+
 }  // namespace pbe
