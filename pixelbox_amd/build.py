@@ -12,10 +12,12 @@ source's.  The translation units compile in parallel.
 from __future__ import annotations
 
 import hashlib
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -29,6 +31,9 @@ HEADERS = ["pb_common.h", "pb_scan_kernels.h", "pb_embed_common.h", "pb_embed_ke
 # host pass of hipcc warns that it does not know the feature: harmless)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall",
          "-Wno-unused-function", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# the short way from torch tensors to the linear layers' entry points (pixelbox_amd/linear.py): host code, against torch's headers
+CALL_SRC = "pb_linear_call.cpp"
+CALL_LIB = os.path.join(HERE, "_linear_call.so")
 # RCCL (the sharded index's all-gather, pb_sharded.hip) is dlopen'ed at pb_sharded_create: a single-GPU host never loads it
 LINK = ["-ldl"]
 
@@ -47,7 +52,7 @@ def _extra() -> list[str]:
 def source_hash() -> str:
     h = hashlib.sha256()
     h.update(" ".join(FLAGS + _extra() + LINK).encode())
-    for rel in SOURCES + HEADERS:
+    for rel in SOURCES + HEADERS + [CALL_SRC]:
         p = os.path.join(CSRC, rel)
         if os.path.exists(p):
             h.update(rel.encode())
@@ -56,8 +61,13 @@ def source_hash() -> str:
     return h.hexdigest()
 
 
+def _torch_dir() -> str | None:
+    spec = importlib.util.find_spec("torch")
+    return os.path.dirname(spec.origin) if spec and spec.origin else None
+
+
 def needs_build() -> bool:
-    if not (os.path.exists(LIB) and os.path.exists(STAMP)):
+    if not (os.path.exists(LIB) and os.path.exists(STAMP)) or (_torch_dir() and not os.path.exists(CALL_LIB)):
         return True
     with open(STAMP) as f:
         return f.read().strip() != source_hash()
@@ -72,6 +82,21 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def _build_call(verbose: bool) -> bool:
+    """_linear_call.so; False where there is no torch to build it against (a host without Python has no use for it)"""
+    t = _torch_dir()
+    if t is None:
+        return False
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-I" + os.path.join(t, "include"),
+           "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I/opt/rocm/include", "-I" + sysconfig.get_paths()["include"],
+           os.path.join(CSRC, CALL_SRC), "-o", CALL_LIB, "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
+           "-Wl,-rpath," + os.path.join(t, "lib")]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.check_call(cmd)
+    return True
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     want = source_hash()
     if not force and not needs_build():
@@ -79,7 +104,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
     with ThreadPoolExecutor(max_workers=min(5, len(srcs))) as ex:
+        call = ex.submit(_build_call, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
+        has_call = call.result()
     cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + LINK
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
@@ -87,7 +114,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with open(STAMP, "w") as f:
         f.write(want + "\n")
     print(f"pixelbox_amd.build: compiled {len(srcs)} translation units for gfx950 -> {os.path.basename(LIB)} "
-          f"(sha256 of sources + flags {want[:16]})", file=sys.stderr)
+          f"{'and _linear_call.so ' if has_call else ''}(sha256 of sources + flags {want[:16]})", file=sys.stderr)
     return LIB
 
 

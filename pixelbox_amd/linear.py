@@ -15,6 +15,8 @@ operand that requires one is refused.
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from . import capi
@@ -39,8 +41,25 @@ def _device(t: torch.Tensor, name: str) -> int:
     return index
 
 
-# One call of these operators is a kernel of a few microseconds, so the usual tensor -- right type, shape and device, contiguous -- passes in
-# one comparison each; only what fails it is looked at closely.
+# One call of these operators is a kernel of a few microseconds; checks from Python and ctypes take as long again.  _linear_call (csrc/
+# pb_linear_call.cpp, built beside the library) looks at the usual call -- plain contiguous tensors of the right types, shapes and device -- and
+# makes it; it answers None for any other, which is then checked here, name by name, and made through ctypes.
+_compiled = None
+
+
+def _load():
+    global _compiled
+    L = capi.lib()
+    try:
+        from . import _linear_call
+    except ImportError:  # built without torch's headers: the calls below do the same
+        _compiled = False
+    else:
+        _linear_call.bind(*(C.cast(f, C.c_void_p).value for f in (L.pb_quantize_rows, L.pb_linear_i8, L.pb_group_rows, L.pb_linear_grouped)))
+        _compiled = _linear_call
+    return _compiled
+
+
 def _check(t: torch.Tensor, name: str, shape: tuple, dtypes: tuple, index: int) -> None:
     """dtype, device, shape (None: any length) and a contiguous last axis"""
     if t.dtype in dtypes and t.get_device() == index and t.shape == shape and t.is_contiguous():
@@ -93,6 +112,13 @@ def _call(rc: int) -> None:
 def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scale: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """x [m, k] (f32, bf16, f16) -> (codes int8 [m, k], scale f32 [m]): scale = max(max |x| / 127, 2^-126) of each row, codes rounded to the
     nearest, halves to even.  A row with an infinity or a NaN has scale NaN and codes 0."""
+    short = _load() if _compiled is None else _compiled
+    if short and codes is not None and scale is not None:
+        rc = short.quantize_rows(x, codes, scale)
+        if rc == 0:
+            return codes, scale
+        if rc is not None:
+            _call(rc)
     dev = _device(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x has the shape {tuple(x.shape)}, not (rows, values)")
@@ -116,8 +142,15 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
               dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
     """act((x w^T) * x_scale * w_scale + bias): x int8 [m, k], w int8 [n, k], x_scale f32 [m], w_scale f32 [n], bias f32 [n].  The result has
     `dtype`, or out's."""
-    dev = _device(x, "x")
     code = _act(act)
+    short = _load() if _compiled is None else _compiled
+    if short and out is not None:
+        rc = short.linear_i8(x, x_scale, w, w_scale, bias, code, out)
+        if rc == 0:
+            return out
+        if rc is not None:
+            _call(rc)
+    dev = _device(x, "x")
     if x.dim() != 2 or w.dim() != 2:
         raise ValueError(f"x and w have the shapes {tuple(x.shape)} and {tuple(w.shape)}, not (m, k) and (n, k)")
     m, k = x.shape
@@ -144,6 +177,13 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
 def group_rows(group: torch.Tensor, groups: int, offsets: torch.Tensor | None = None, order: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """group int32 [m] -> (offsets int32 [groups + 1], order int32 [m]): group g's rows are order[offsets[g] : offsets[g + 1]], ascending.  Rows with a
     group outside [0, groups) come last, behind offsets[groups]."""
+    short = _load() if _compiled is None else _compiled
+    if short and offsets is not None and order is not None:
+        rc = short.group_rows(group, groups, offsets, order)
+        if rc == 0:
+            return offsets, order
+        if rc is not None:
+            _call(rc)
     dev = _device(group, "group")
     if group.dim() != 1:
         raise ValueError(f"group has the shape {tuple(group.shape)}, not (rows,)")
@@ -172,8 +212,19 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     [groups + 1].  x_rows and y_rows (int32 [m], `rows` for both) name the row of x that is read and the row of out that is written at each place r;
     without them it is r itself.  Rows of out that no place names are left as they are: zero where out is made here (m rows, or as many as x has
     where y_rows is given)."""
-    dev = _device(x, "x")
     code = _act(act)
+    if rows is not None:
+        if x_rows is not None or y_rows is not None:
+            raise ValueError("rows stands for x_rows and y_rows: give one or the other")
+        x_rows = y_rows = rows
+    short = _load() if _compiled is None else _compiled
+    if short and out is not None:
+        rc = short.linear_grouped(x, w, offsets, x_rows, y_rows, x_scale, w_scale, bias, code, out)
+        if rc == 0:
+            return out
+        if rc is not None:
+            _call(rc)
+    dev = _device(x, "x")
     if x.dim() != 2 or w.dim() != 3:
         raise ValueError(f"x and w have the shapes {tuple(x.shape)} and {tuple(w.shape)}, not (rows, k) and (groups, n, k)")
     x_total, k = x.shape
@@ -188,10 +239,6 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
         if ldw < k or (groups > 1 and n > 0 and w.stride(0) != n * ldw):
             raise ValueError("w: the groups' weights do not follow one another row by row")
     _check(offsets, "offsets", (groups + 1,), (torch.int32,), dev)
-    if rows is not None:
-        if x_rows is not None or y_rows is not None:
-            raise ValueError("rows stands for x_rows and y_rows: give one or the other")
-        x_rows = y_rows = rows
     m = x_total
     if x_rows is not None:
         m = x_rows.numel()

@@ -465,3 +465,56 @@ def test_no_gradient_is_refused_not_lost():
         linear.quantize_rows(x)
     with torch.no_grad():
         assert linear.linear_grouped(x, w, offsets).shape == (4, 5)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_the_short_call_is_taken_and_gives_the_same(kind, monkeypatch):
+    """pixelbox_amd/_linear_call.so takes the usual calls; without it the same calls go through ctypes"""
+    assert linear._load(), "pixelbox_amd/_linear_call.so is not built"
+    m, groups, n, k = 100, 3, 40, 64
+    x, xs, w, ws, b = grouped_case(kind, m, groups, n, k, 90)
+    xf, group = rand((m, k), torch.float32, gen(91)), some_groups(m, groups, 92)
+
+    def everything():
+        offsets, order = torch.empty(groups + 1, dtype=torch.int32, device="cuda"), torch.empty(m, dtype=torch.int32, device="cuda")
+        c, s = torch.empty((m, k), dtype=torch.int8, device="cuda"), torch.empty(m, device="cuda")
+        linear.group_rows(group, groups, offsets=offsets, order=order)
+        linear.quantize_rows(xf, codes=c, scale=s)
+        y = linear.linear_grouped(x, w, offsets, rows=order, x_scale=xs, w_scale=ws, bias=b, act="silu", out=torch.zeros((m, n), device="cuda"))
+        got = [offsets, order, c, s, y]
+        if kind == "i8":
+            got.append(linear.linear_i8(x, xs, w[0], ws[0], bias=b[0], out=torch.empty((m, n), dtype=torch.float16, device="cuda")))
+        return got
+
+    taken = []
+
+    class Counting:
+        def __getattr__(self, name):
+            f = getattr(linear._load(), name)
+
+            def call(*a):
+                rc = f(*a)
+                taken.append((name, rc))
+                return rc
+            return call
+
+    short = linear._load()
+    monkeypatch.setattr(linear, "_load", lambda: short)
+    monkeypatch.setattr(linear, "_compiled", Counting())
+    first = everything()
+    assert all(rc == 0 for _, rc in taken) and len(taken) == len(first) - 2, taken
+    monkeypatch.setattr(linear, "_compiled", False)
+    assert all(torch.equal(a, b) for a, b in zip(first, everything()))
+
+
+def test_the_short_call_leaves_the_unusual_alone():
+    short = linear._load()
+    x, xs, w, ws, b = i8_case(6, 8, 32, 1)
+    out = torch.empty((6, 8), device="cuda")
+    ok = [x, xs, w, ws, b, 0, out]
+    assert short.linear_i8(*ok) == 0
+    for i, odd in ((0, x.cpu()), (0, x.float()), (1, xs[:5]), (2, w.t()), (3, None), (4, b.double()), (6, out.t()), (6, out[:, :7]), (0, None)):
+        assert short.linear_i8(*ok[:i], odd, *ok[i + 1:]) is None, i
+    assert short.linear_i8(x, xs, w, ws, b, 7, out) == -1  # the library's own refusal
+    with pytest.raises(capi.PixelboxError):
+        linear.linear_i8(x, xs, w, ws, out=x.view(torch.float32)[:, :8].as_strided((6, 8), (8, 1)))  # y over x
