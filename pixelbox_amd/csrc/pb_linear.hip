@@ -95,9 +95,9 @@ int launch(LinearArgs a, hipStream_t s) {
     a.n_tiles = (int)n_tiles;
     const dim3 grid((unsigned)((row_tiles * n_tiles + 7) / 8 * 8));
     switch (f) {
-        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
-        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
-        case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2, ALIGNED>), grid, dim3(512), 0, s, a); break;
+        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4>), grid, dim3(512), 0, s, a); break;
+        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4>), grid, dim3(512), 0, s, a); break;
+        case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2>), grid, dim3(512), 0, s, a); break;
         case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, ALIGNED ? 4 : 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
         case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
         case TILE128W: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 64, 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
@@ -157,7 +157,7 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     a.ldx = (long)ldx * size;
     a.ldw = (long)ldw * size;
     a.ldy = (long)ldy * y_size;
-    a.kb = (long)k * size;
+    a.kb = (int)k * size;
     a.m = (int)m;
     a.n = (int)n;
     a.groups = (int)groups;
@@ -166,7 +166,6 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     a.y_total = (int)y_total;
     a.act = act;
     a.y_type = y_type;
-    a.y_vec = !misaligned(y, 16) && a.ldy % 16 == 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (type) {
         case PB_TYPE_F32: return launch<F32>(a, s);
@@ -177,14 +176,14 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
 }
 
 // a wave per row where the row fits its registers and there are rows for every CU, else a workgroup of four
-template <int T, bool VEC>
+template <int T>
 void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale, hipStream_t s) {
     const uint8_t *px = static_cast<const uint8_t *>(x);
     int8_t *pc = static_cast<int8_t *>(codes);
     constexpr uint32_t V = T == F32 ? 4 : 8;
     const long lx = (long)ldx * type_bytes(T), lc = (long)ldc;
-    if (m >= 1024 && k <= 64 * V * 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 8, VEC>), dim3((unsigned)((m + 3) / 4)), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
-    else hipLaunchKernelGGL((k_quantize_rows<T, 256, 4, VEC>), dim3((unsigned)m), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
+    if (m >= 1024 && k <= 64 * V * 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 8>), dim3((unsigned)((m + 3) / 4)), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
+    else hipLaunchKernelGGL((k_quantize_rows<T, 256, 4>), dim3((unsigned)m), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
 }
 
 }  // namespace
@@ -205,12 +204,10 @@ int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int v = x_type == PB_TYPE_F32 ? 4 : 8;
-    const bool vec = !misaligned(x, 16) && ldx * size % 16 == 0 && !misaligned(codes, v) && ldc % v == 0;
     switch (x_type) {
-        case PB_TYPE_F32: vec ? launch_quantize<F32, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<F32, false>(x, m, k, ldx, codes, ldc, scale, s); break;
-        case PB_TYPE_BF16: vec ? launch_quantize<BF16, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<BF16, false>(x, m, k, ldx, codes, ldc, scale, s); break;
-        default: vec ? launch_quantize<F16, true>(x, m, k, ldx, codes, ldc, scale, s) : launch_quantize<F16, false>(x, m, k, ldx, codes, ldc, scale, s); break;
+        case PB_TYPE_F32: launch_quantize<F32>(x, m, k, ldx, codes, ldc, scale, s); break;
+        case PB_TYPE_BF16: launch_quantize<BF16>(x, m, k, ldx, codes, ldc, scale, s); break;
+        default: launch_quantize<F16>(x, m, k, ldx, codes, ldc, scale, s); break;
     }
     PB_HIP(hipGetLastError());
     return PB_OK;

@@ -64,28 +64,24 @@ __device__ __forceinline__ void mma32(typename Acc<T>::q16 &c, const u32x4 &a, c
     }
 }
 
-// ---- loads ------------------------------------------------------------------------------------------------------------------------
-template <bool ALIGNED>
+// ---- loads and stores of any alignment ---------------------------------------------------------------------------------------------------
+// global_load / store_dwordx4 take any address; aligned ones are not slower for it.
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) {
     u32x4 v;
-    if constexpr (ALIGNED) v = *reinterpret_cast<const u32x4 *>(p);
-    else __builtin_memcpy(&v, p, 16);  // global_load_dwordx4 takes any address
+    __builtin_memcpy(&v, p, 16);
     return v;
 }
-// bytes [at, at + 16) of a row of `len` bytes, zero behind its end; reads nothing outside [0, len)
-template <bool ALIGNED>
-__device__ __forceinline__ u32x4 load16_tail(const uint8_t *row, long at, long len) {
-    if (at + 16 <= len) return load16<ALIGNED>(row + at);
-    u32x4 v = {0u, 0u, 0u, 0u};
-    if (at >= len) return v;
-    if (len >= 16) {  // the row's last 16 bytes, shifted down
-        const u32x4 t = load16<false>(row + len - 16);
-        const int s = 8 * (int)(at + 16 - len);  // 8 .. 120 bits
+__device__ __forceinline__ void store16(uint8_t *p, const u32x4 &v) { __builtin_memcpy(p, &v, 16); }
+// bytes [at, at + 16) of a row of `len` bytes, zero behind its end; reads nothing outside [0, len).  Without a branch for rows of 16
+// bytes and more, so that several such loads are on their way together: the row's last 16 bytes, shifted down.
+__device__ __forceinline__ u32x4 load16_tail(const uint8_t *row, int at, int len) {
+    if (len >= 16) {
+        const int off = min(at, len - 16), s = 8 * (at - off);
+        const u32x4 t = load16(row + off);
         const uint64_t lo = ((uint64_t)t.y << 32) | t.x, hi = ((uint64_t)t.w << 32) | t.z;
-        const uint64_t l2 = s >= 64 ? hi >> (s - 64) : (lo >> s) | (hi << (64 - s));
-        const uint64_t h2 = s >= 64 ? 0 : hi >> s;
-        v = {(uint32_t)l2, (uint32_t)(l2 >> 32), (uint32_t)h2, (uint32_t)(h2 >> 32)};
-        return v;
+        const uint64_t l2 = s == 0 ? lo : s < 64 ? (lo >> s) | (hi << (64 - s)) : s < 128 ? hi >> (s - 64) : 0;
+        const uint64_t h2 = s < 64 ? hi >> s : 0;
+        return u32x4{(uint32_t)l2, (uint32_t)(l2 >> 32), (uint32_t)h2, (uint32_t)(h2 >> 32)};
     }
     uint64_t half[2] = {0, 0};  // rows shorter than one piece
 #pragma unroll 1
@@ -94,8 +90,7 @@ __device__ __forceinline__ u32x4 load16_tail(const uint8_t *row, long at, long l
         half[0] |= i < 8 ? b : 0;
         half[1] |= i < 8 ? 0 : b;
     }
-    v = {(uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32)};
-    return v;
+    return u32x4{(uint32_t)half[0], (uint32_t)(half[0] >> 32), (uint32_t)half[1], (uint32_t)(half[1] >> 32)};
 }
 
 // ---- arguments of a product -----------------------------------------------------------------------------------------------------------
@@ -105,11 +100,10 @@ struct LinearArgs {
     const int32_t *offsets, *x_rows, *y_rows;
     uint8_t *y;
     long ldx, ldw, ldy;      // bytes between rows
-    long kb;                 // bytes summed over
+    int kb;                  // bytes summed over (k <= 2^28)
     int m, n, groups, n_tiles;
     int x_total, y_total;    // rows of x and y: an index outside them is no row
     int act, y_type;
-    int y_vec;               // rows of y start on 16 bytes
 };
 
 // ---- which rows a workgroup works on ----------------------------------------------------------------------------------------------------
@@ -212,13 +206,11 @@ template <int W>
 __device__ __forceinline__ void store_row(const LinearArgs &a, int yr, int c0, const float (&v)[W]) {
     if (c0 >= a.n) return;
     uint8_t *row = a.y + (long)yr * a.ldy;
-    const bool whole = a.y_vec && c0 + W <= a.n;
+    const bool whole = c0 + W <= a.n;
     if (a.y_type == F32) {
         float *p = reinterpret_cast<float *>(row) + c0;
-        if (whole) {
-#pragma unroll
-            for (int i = 0; i < W; i += 4) *reinterpret_cast<f32x4 *>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-        } else {
+        if (whole) __builtin_memcpy(p, v, 4 * W);
+        else {
 #pragma unroll
             for (int i = 0; i < W; ++i)
                 if (c0 + i < a.n) p[i] = v[i];
@@ -228,10 +220,8 @@ __device__ __forceinline__ void store_row(const LinearArgs &a, int yr, int c0, c
         uint32_t h[W / 2];
 #pragma unroll
         for (int i = 0; i < W / 2; ++i) h[i] = pack2(v[2 * i], v[2 * i + 1], a.y_type);
-        if (whole) {
-            if constexpr (W == 8) *reinterpret_cast<u32x4 *>(p) = u32x4{h[0], h[1], h[2], h[3]};
-            else *reinterpret_cast<u32x2 *>(p) = u32x2{h[0], h[1]};
-        } else {
+        if (whole) __builtin_memcpy(p, h, 2 * W);
+        else {
 #pragma unroll
             for (int i = 0; i < W; ++i)
                 if (c0 + i < a.n) p[i] = (uint16_t)(h[i / 2] >> (16 * (i & 1)));
@@ -242,7 +232,7 @@ __device__ __forceinline__ void store_row(const LinearArgs &a, int yr, int c0, c
 // what a lane needs of its W output channels
 template <int T, int W> struct Chan {
     float scale[W], bias[W];
-    __device__ __forceinline__ Chan(const LinearArgs &a, int g, int c0) {
+    __device__ __forceinline__ void load(const LinearArgs &a, int g, int c0) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
             const bool in = c0 + i < a.n;
@@ -263,14 +253,10 @@ template <int T, int W> struct Chan {
             if constexpr (!PLAIN) v[i] = act_f(v[i], a.act);
         }
         if constexpr (!PLAIN) store_row<W>(a, yr, c0, v);
-        else if constexpr (YT == F32) {
-            float *p = reinterpret_cast<float *>(a.y + (long)yr * a.ldy) + c0;
-#pragma unroll
-            for (int i = 0; i < W; i += 4) *reinterpret_cast<f32x4 *>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
-        } else {
+        else if constexpr (YT == F32) __builtin_memcpy(reinterpret_cast<float *>(a.y + (long)yr * a.ldy) + c0, v, 4 * W);
+        else {
             static_assert(W == 8, "");
-            *reinterpret_cast<u32x4 *>(reinterpret_cast<uint16_t *>(a.y + (long)yr * a.ldy) + c0) =
-                u32x4{pack2(v[0], v[1], YT), pack2(v[2], v[3], YT), pack2(v[4], v[5], YT), pack2(v[6], v[7], YT)};
+            store16(a.y + (long)yr * a.ldy + 2 * c0, u32x4{pack2(v[0], v[1], YT), pack2(v[2], v[3], YT), pack2(v[4], v[5], YT), pack2(v[6], v[7], YT)});
         }
     }
 };
@@ -334,11 +320,10 @@ __device__ __forceinline__ void store_rows(const LinearArgs &a, const Chan<T, 8>
     }
 }
 template <int T, int MT, int NT, int WN>
-__device__ __forceinline__ void store_tile(const LinearArgs &a, int g, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem, const int *yrows,
-                                           const float *scales, int wave, int lane, int c_wave, int valid) {
+__device__ __forceinline__ void store_tile(const LinearArgs &a, const Chan<T, 8> &ch, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem,
+                                           const int *yrows, const float *scales, int wave, int lane, int c_wave, int valid) {
     const int c0 = c_wave + (lane % (WN / 8)) * 8;
-    const Chan<T, 8> ch(a, g, c0);
-    const bool plain = a.act == PB_ACT_NONE && a.y_vec && c_wave + WN <= a.n;  // of the whole wave
+    const bool plain = a.act == PB_ACT_NONE && c_wave + WN <= a.n;  // of the whole wave
     if (plain && a.y_type == BF16) store_rows<T, MT, NT, WN, true, BF16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
     else if (plain && a.y_type == F16) store_rows<T, MT, NT, WN, true, F16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
     else if (plain) store_rows<T, MT, NT, WN, true, F32>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
@@ -383,30 +368,36 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
         const int row = ((tid + j * NTHR) >> 3);
         pp[j] = (j < JA ? a.x + (long)max(s_xrow[j < JA ? row : 0], 0) * a.ldx : a.w + ((long)t.g * a.n + min(c_base + row - BM, a.n - 1)) * a.ldw) + lc;
     }
-    const int full = (int)(a.kb >> 7), steps = (int)((a.kb + 127) >> 7);
+    const int full = a.kb >> 7, steps = (a.kb + 127) >> 7;
     auto stage = [&](int i) { return s_mem + (i & (NST - 1)) * STAGE; };
     auto dma = [&](int i, int j) {
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pp[j] + (long)i * 128),
                                          (__attribute__((address_space(3))) void *)(stage(i) + wave * 1024 + j * NTHR * 16), 16, 0, 0);
     };
     auto copy_tail = [&](int i) {  // the partial step behind the full ones
-#pragma unroll 1
-        for (int j = 0; j < J; ++j) {
-            const uint8_t *row = j < JA ? a.x + (long)max(s_xrow[(tid + j * NTHR) >> 3], 0) * a.ldx
-                                        : a.w + ((long)t.g * a.n + min(c_base + ((tid + j * NTHR) >> 3) - BM, a.n - 1)) * a.ldw;
-            *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = load16_tail<DMA>(row, (long)i * 128 + lc, a.kb);
+#pragma unroll
+        for (int j0 = 0; j0 < J; j0 += 4) {  // four loads on their way at a time
+            u32x4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4 && j0 + j < J; ++j) v[j] = load16_tail(pp[j0 + j] - lc, i * 128 + lc, a.kb);
+#pragma unroll
+            for (int j = 0; j < 4 && j0 + j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + (j0 + j) * NTHR) * 16) = v[j];
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     u32x4 regs[DMA ? 1 : J];
     auto load_regs = [&](int i, u32x4 (&to)[DMA ? 1 : J]) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) to[DMA ? 0 : j] = load16<false>(pp[j] + (long)i * 128);
+        for (int j = 0; j < J; ++j) to[DMA ? 0 : j] = load16(pp[j] + (long)i * 128);
     };
     auto put_regs = [&](int i, const u32x4 (&from)[DMA ? 1 : J]) {
 #pragma unroll
         for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = from[DMA ? 0 : j];
     };
     const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 31, hi = lane >> 5;
+    constexpr bool EARLY = MT * NT < 8;  // registers for them: on their way under the product
+    Chan<T, 8> ch;
+    if constexpr (EARLY) ch.load(a, t.g, c_base + wn + (lane % (WN / 8)) * 8);
     typename Acc<T>::q16 acc[NT][MT] = {};
     const uint8_t *sa = s_mem + (wm + li) * 128, *sb = s_mem + (BM + wn + li) * 128;
     u32x4 fa[NF][MT], fb[NF][NT];
@@ -525,14 +516,15 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
     if (valid <= 0) walk(std::integral_constant<int, 0>{});
     else if (MT > 1 && valid <= WM / 2) walk(std::integral_constant<int, (MT > 1 ? MT / 2 : MT)>{});
     else walk(std::integral_constant<int, MT>{});
+    if constexpr (!EARLY) ch.load(a, t.g, c_base + wn + (lane % (WN / 8)) * 8);
     __syncthreads();  // the stages become the waves' epilogue images
-    store_tile<T, MT, NT, WN>(a, t.g, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn, valid);
+    store_tile<T, MT, NT, WN>(a, ch, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn, valid);
 }
 
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
 // For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
 // waves' partial sums meet in LDS and are added in wave order.
-template <int T, int MT, int NT, int NW, int U, bool ALIGNED>
+template <int T, int MT, int NT, int NW, int U>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     typedef typename Acc<T>::e E;
     typedef typename Acc<T>::q4 Q;
@@ -550,24 +542,24 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) pw[j] = a.w + ((long)t.g * a.n + min(c_base + j * 16 + li, a.n - 1)) * a.ldw + kq;
     Q acc[NT][MT] = {};
-    const int kb1 = (int)a.kb;
+    const int kb1 = a.kb;
     for (int kb = wave * 64 * U; kb < kb1; kb += 64 * U * NW) {
         u32x4 fw[U][NT], fx[U][MT];
         if (kb + 64 * U <= kb1) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16<ALIGNED>(pw[j] + kb + u * 64);
+                for (int j = 0; j < NT; ++j) fw[u][j] = load16(pw[j] + kb + u * 64);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16<ALIGNED>(px[i] + kb + u * 64);
+                for (int i = 0; i < MT; ++i) fx[u][i] = load16(px[i] + kb + u * 64);
             }
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail<ALIGNED>(pw[j] - kq, kb + u * 64 + kq, kb1);
+                for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail(pw[j] - kq, kb + u * 64 + kq, kb1);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail<ALIGNED>(px[i] - kq, kb + u * 64 + kq, kb1);
+                for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail(px[i] - kq, kb + u * 64 + kq, kb1);
             }
         }
 #pragma unroll
@@ -594,7 +586,8 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
         }
         const int xr = x_row_of(a, t.r0 + r), yr = y_row_of(a, t.r0 + r);
         if (xr < 0 || yr < 0) continue;
-        const Chan<T, 4> ch(a, t.g, c_base + c);
+        Chan<T, 4> ch;
+        ch.load(a, t.g, c_base + c);
         const E e[4] = {s[0], s[1], s[2], s[3]};
         ch.finish(a, e, T == I8 ? a.x_scale[xr] : 1.0f, yr, c_base + c);
     }
@@ -650,9 +643,8 @@ template <int T> __device__ __forceinline__ float elem(const uint8_t *row, long 
 }
 
 // NTHR threads per row (a wave or a workgroup of four), V values per thread and turn; rows of up to NTHR * V * TURNS values stay in
-// registers between the maximum and the codes, longer ones are read a second time.  VEC: 16-byte loads (rows start on 16 bytes,
-// codes on V).
-template <int T, int NTHR, int TURNS, bool VEC>
+// registers between the maximum and the codes, longer ones are read a second time.
+template <int T, int NTHR, int TURNS>
 __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict__ x, int m, int k, long ldx, int8_t *__restrict__ codes, long ldc,
                                                        float *__restrict__ scale) {
     constexpr int V = T == F32 ? 4 : 8, RPB = 256 / NTHR;
@@ -664,8 +656,8 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
     int8_t *pc = codes + (long)row * ldc;
     const uint32_t INF = 0x7f800000u;
     auto load = [&](int c, float (&v)[V]) {
-        if (VEC && c + V <= k) {
-            const u32x4 q = *reinterpret_cast<const u32x4 *>(px + (long)c * type_bytes(T));
+        if (c + V <= k) {
+            const u32x4 q = load16(px + (long)c * type_bytes(T));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if constexpr (T == F32) v[i] = __uint_as_float(q[i]);
@@ -709,7 +701,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
         }
         uint32_t w[V / 4];
         codes_of<V>(u, inv, sc, half, w);
-        if (VEC && c + V <= k) __builtin_memcpy(__builtin_assume_aligned(pc + c, V), w, V);
+        if (c + V <= k) __builtin_memcpy(pc + c, w, V);
         else {
 #pragma unroll
             for (int i = 0; i < V; ++i)
