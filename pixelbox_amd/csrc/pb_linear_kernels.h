@@ -157,32 +157,34 @@ __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
         }
     } else m_tiles = (a.m + BM - 1) / BM;
     Tile t = {0, 0, 0, 0};
-    // workgroups go round robin over the 8 XCDs: XCD x takes a contiguous eighth of the tiles, so that its L2 sees few panels.
-    // Inside it, BAND row tiles go through the channel tiles together.
+    // workgroups go round robin over the 8 XCDs: XCD x takes a contiguous eighth of the tiles, so that its L2 sees few panels.  A
+    // group's tiles follow one another; inside it, BAND row tiles go through the channel tiles together.
     const long total = m_tiles * a.n_tiles, per = (total + 7) / 8;
-    const long b = blockIdx.x, in = b >> 3, id = (b & 7) * per + in;
+    const long b = blockIdx.x, in = b >> 3;
+    long id = (b & 7) * per + in;
     if (in >= per || id >= total) return t;
-    const long band = id / ((long)BAND * a.n_tiles), rest = id - band * BAND * a.n_tiles;
-    const int bh = (int)min((long)BAND, m_tiles - band * BAND);
-    t.nt = (int)(rest / bh);
-    int mt = (int)(band * BAND + rest % bh);
-    if (!a.offsets) {
-        t.r0 = mt * BM;
-        t.r1 = min(t.r0 + BM, a.m);
-        return t;
-    }
-    for (int g0 = 0; g0 < a.groups; g0 += 64) {
-        if (a.groups > 64) look(g0);
-        const uint64_t past = __ballot(inc > mt);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            t.g = g0 + l;
-            t.r0 = __builtin_amdgcn_readlane(lo, l) + (mt - __builtin_amdgcn_readlane(inc - c, l)) * BM;
-            t.r1 = min(t.r0 + BM, __builtin_amdgcn_readlane(hi, l));
-            return t;
+    int lo_g = 0, hi_g = a.m, tiles_g = (int)m_tiles;
+    if (a.offsets) {
+        for (int g0 = 0; g0 < a.groups; g0 += 64) {
+            if (a.groups > 64) look(g0);
+            const uint64_t past = __ballot((long)inc * a.n_tiles > id);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                t.g = g0 + l;
+                lo_g = __builtin_amdgcn_readlane(lo, l);
+                hi_g = __builtin_amdgcn_readlane(hi, l);
+                tiles_g = __builtin_amdgcn_readlane(c, l);
+                id -= (long)(__builtin_amdgcn_readlane(inc, l) - tiles_g) * a.n_tiles;
+                break;
+            }
+            id -= (long)__builtin_amdgcn_readlane(inc, 63) * a.n_tiles;
         }
-        mt -= __builtin_amdgcn_readlane(inc, 63);
     }
+    const int band = (int)(id / ((long)BAND * a.n_tiles));
+    const int rest = (int)(id - (long)band * BAND * a.n_tiles), bh = min(BAND, tiles_g - band * BAND);
+    t.nt = rest / bh;
+    t.r0 = lo_g + (band * BAND + rest % bh) * BM;
+    t.r1 = min(t.r0 + BM, hi_g);
     return t;
 }
 
