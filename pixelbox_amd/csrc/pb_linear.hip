@@ -100,9 +100,9 @@ int launch(LinearArgs a, hipStream_t s) {
         case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2>), grid, dim3(512), 0, s, a); break;
         case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, ALIGNED ? 4 : 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
         case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
-        case TILE128W: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 64, 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
+        case TILE128W: hipLaunchKernelGGL((k_linear_wide<T, 128, 128, 64, 64, 2, 3, ALIGNED>), grid, dim3(256), 0, s, a); break;
         default:
-            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_tile<T, 256, 256, 128, 64, 2, ALIGNED>), grid, dim3(512), 0, s, a);
+            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_wide<T, 256, 256, 128, 64, 2, ALIGNED ? 7 : 1, ALIGNED>), grid, dim3(512), 0, s, a);
             break;
     }
     PB_HIP(hipGetLastError());

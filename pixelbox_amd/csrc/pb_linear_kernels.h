@@ -289,27 +289,22 @@ __device__ __forceinline__ void rows_to_lds(const LinearArgs &a, const Tile &t, 
     }
 }
 
-// A wave's sums -> y, 32 rows x WN channels at a time: they go to LDS as the matrix instruction left them (4 consecutive channels per
-// lane) and come back as 8 consecutive channels per lane, whole rows by consecutive lanes.  s_mem: 32 (WN + 4) sums for each wave.
-template <int T, int MT, int NT, int WN, bool PLAIN, int YT>
-__device__ __forceinline__ void store_rows(const LinearArgs &a, const Chan<T, 8> &ch, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem,
-                                           const int *yrows, const float *scales, int wave, int lane, int c0, int valid) {
+// A wave's sums -> y, 32 rows x WN channels at a time: image(img, i) puts the sums of rows 32 i .. + 32 into LDS as the matrix
+// instruction left them (4 consecutive channels per lane), and they come back as 8 consecutive channels per lane, whole rows by
+// consecutive lanes.  s_mem: 32 (WN + 4) sums for each wave.
+template <int T, int R, int WN, bool PLAIN, int YT, class Image>
+__device__ __forceinline__ void store_rows(const LinearArgs &a, const Chan<T, 8> &ch, Image &&image, uint8_t *s_mem, const int *yrows, const float *scales,
+                                           int wave, int lane, int c0, int valid) {
     typedef typename Acc<T>::e E;
     typedef typename Acc<T>::q4 Q;
     constexpr int PITCH = WN + 4;
     E *img = reinterpret_cast<E *>(s_mem) + wave * 32 * PITCH;
     constexpr int LPR = WN / 8, RPI = 64 / LPR;  // lanes per row, rows per instruction
-    const int li = lane & 31, hi = lane >> 5, c8 = (lane % LPR) * 8;
+    const int c8 = (lane % LPR) * 8;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < R; ++i) {
         if (i * 32 >= valid) break;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const Q v = {acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
-                *reinterpret_cast<Q *>(img + li * PITCH + j * 32 + q * 8 + hi * 4) = v;
-            }
+        image(img, i);
         __builtin_amdgcn_wave_barrier();  // one wave's LDS accesses are in order
 #pragma unroll
         for (int r = 0; r < 32; r += RPI) {
@@ -321,40 +316,112 @@ __device__ __forceinline__ void store_rows(const LinearArgs &a, const Chan<T, 8>
         __builtin_amdgcn_wave_barrier();
     }
 }
-template <int T, int MT, int NT, int WN>
-__device__ __forceinline__ void store_tile(const LinearArgs &a, const Chan<T, 8> &ch, const typename Acc<T>::q16 (&acc)[NT][MT], uint8_t *s_mem,
-                                           const int *yrows, const float *scales, int wave, int lane, int c_wave, int valid) {
+template <int T, int R, int WN, class Image>
+__device__ __forceinline__ void store_tile(const LinearArgs &a, const Chan<T, 8> &ch, Image &&image, uint8_t *s_mem, const int *yrows, const float *scales,
+                                           int wave, int lane, int c_wave, int valid) {
     const int c0 = c_wave + (lane % (WN / 8)) * 8;
     const bool plain = a.act == PB_ACT_NONE && c_wave + WN <= a.n;  // of the whole wave
-    if (plain && a.y_type == BF16) store_rows<T, MT, NT, WN, true, BF16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
-    else if (plain && a.y_type == F16) store_rows<T, MT, NT, WN, true, F16>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
-    else if (plain) store_rows<T, MT, NT, WN, true, F32>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
-    else store_rows<T, MT, NT, WN, false, F32>(a, ch, acc, s_mem, yrows, scales, wave, lane, c0, valid);
+    if (plain && a.y_type == BF16) store_rows<T, R, WN, true, BF16>(a, ch, image, s_mem, yrows, scales, wave, lane, c0, valid);
+    else if (plain && a.y_type == F16) store_rows<T, R, WN, true, F16>(a, ch, image, s_mem, yrows, scales, wave, lane, c0, valid);
+    else if (plain) store_rows<T, R, WN, true, F32>(a, ch, image, s_mem, yrows, scales, wave, lane, c0, valid);
+    else store_rows<T, R, WN, false, F32>(a, ch, image, s_mem, yrows, scales, wave, lane, c0, valid);
 }
 
-// ---- k_linear_tile: a tile of BM rows x BN channels per workgroup, K in steps of 128 bytes through LDS ------------------------------------
-// A step has four pieces of 32 bytes of K; a piece's fragments are read from LDS while the one before is multiplied.  The one barrier
-// of a step stands before its LAST piece, whose fragments are in registers by then: behind it the step's stage is free, so the loads
-// of step i + NST leave there (NST LDS stages) and have NST - 1 steps to arrive, and the first fragments of step i + 1 are read while
-// the last piece of step i is multiplied -- the matrix pipe has work across the barrier.  Waves with one or two matrix instructions
-// to a piece (FLAT) would wait out an LDS read for each piece: they read all four at once behind the barrier.
-// Rows sit in LDS at a pitch of 128 bytes with their eight 16-byte pieces permuted (piece c at c ^ (row / 2 & 7)), which makes the
-// fragment reads (16 bytes from each of 32 rows) free of bank conflicts: 249 bytes a clock and CU, against 121 with c ^ (row & 7)
-// and 32 unpermuted (LDS reads alone, 256 workgroups of eight waves); the permutation is done by the lanes' GLOBAL addresses, so a
-// wave's eight rows of 128 bytes are still whole lines.  DMA: the loads go straight into LDS (16-byte aligned rows); otherwise
-// through registers, which takes any alignment.  The last, partial step always goes through registers.
+// What the tile kernels share: K goes in steps of 128 bytes through NST LDS stages.  A row sits in LDS at a pitch of 128 bytes with its
+// eight 16-byte pieces permuted, so that the fragment reads -- 16 bytes from each of 32 (or of 16 x 4) places -- are free of bank
+// conflicts: with 32-row fragments piece c at c ^ (row / 2 & 7): 249 bytes a clock and CU, against 121 with c ^ (row & 7) and 32
+// unpermuted; with 16-row fragments c ^ (row & 7): 242 (LDS reads alone, 256 workgroups of eight waves).  The permutation is done by
+// the lanes' GLOBAL addresses, so a wave's eight rows of 128 bytes are still whole lines.  DMA: the loads go straight into LDS
+// (16-byte aligned rows); otherwise through registers, which takes any alignment.  The last, partial step always goes through registers.
+template <int T, int BM, int BN, int NTHR, int NST, bool ROWS16>
+struct Loader {
+    static constexpr int TAIL = BM > 128 ? 2 : 4;
+    static constexpr int STAGE = (BM + BN) * 128, JA = BM * 8 / NTHR, J = (BM + BN) * 8 / NTHR;  // 16-byte pieces per thread and step: of x, in all
+    static_assert(BM * 8 % NTHR == 0 && BN * 8 % NTHR == 0 && NTHR / 8 % 16 == 0 && (NST == 2 || NST == 4), "");
+    const uint8_t *pp[J];  // this thread's rows: JA of x, the others of w
+    uint8_t *mem;
+    int tid, wave, lc, kb, full, steps;
+
+    __device__ __forceinline__ Loader(const LinearArgs &a, const Tile &t, uint8_t *s_mem, const int *xrows, int tid_, int wave_) {
+        mem = s_mem;
+        tid = tid_;
+        wave = wave_;
+        kb = a.kb;
+        full = kb >> 7;
+        steps = (kb + 127) >> 7;
+        lc = ((tid & 7) ^ ((tid >> (ROWS16 ? 3 : 4)) & 7)) * 16;  // the piece this thread moves in every row it touches
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int row = (tid + j * NTHR) >> 3;
+            pp[j] = (j < JA ? a.x + (long)max(xrows[j < JA ? row : 0], 0) * a.ldx : a.w + ((long)t.g * a.n + min(t.nt * BN + row - BM, a.n - 1)) * a.ldw) + lc;
+        }
+    }
+    __device__ __forceinline__ uint8_t *stage(int i) const { return mem + (i & (NST - 1)) * STAGE; }
+    __device__ __forceinline__ void dma(int i, int j) const {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pp[j] + (long)i * 128),
+                                         (__attribute__((address_space(3))) void *)(stage(i) + wave * 1024 + j * NTHR * 16), 16, 0, 0);
+    }
+    __device__ __forceinline__ void load(int i, u32x4 (&to)[J]) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j) to[j] = load16(pp[j] + (long)i * 128);
+    }
+    __device__ __forceinline__ void put(int i, const u32x4 (&from)[J]) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = from[j];
+    }
+    __device__ __forceinline__ void tail(int i) const {  // the partial step behind the full ones
+#pragma unroll
+        for (int j0 = 0; j0 < J; j0 += TAIL) {  // a few loads on their way at a time
+            u32x4 v[TAIL];
+#pragma unroll
+            for (int j = 0; j < TAIL && j0 + j < J; ++j) v[j] = load16_tail(pp[j0 + j] - lc, i * 128 + lc, kb);
+#pragma unroll
+            for (int j = 0; j < TAIL && j0 + j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + (j0 + j) * NTHR) * 16) = v[j];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // steps [0, n) before the walk
+    __device__ __forceinline__ void first(int n, bool by_dma) const {
+        for (int i = 0; i < n; ++i) {
+            if (i < full) {
+                if (by_dma) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) dma(i, j);
+                } else {
+                    u32x4 r[J];
+                    load(i, r);
+                    put(i, r);
+                }
+            } else if (i < steps) tail(i);
+        }
+    }
+    // this wave's loads of step i are in LDS; those of younger steps, at most NST - 2 of them, may still be on their way
+    __device__ __forceinline__ void landed(int i) const {
+        const int younger = min(NST - 2, full - 1 - i);
+        if (NST > 3 && younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * J) : "memory");
+        else if (NST > 2 && younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+    static __device__ __forceinline__ void barrier() {  // this wave's LDS reads have come back, its LDS writes are done
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// ---- k_linear_tile: small tiles -- 64 x 64 or 128 x 128, waves of 32 x 32 or 64 x 32 ---------------------------------------------------------
+// For products with few tiles, where a step is short: a wave has one or two 32 x 32 matrix instructions to a 32-byte piece, and would
+// wait out an LDS read for each piece, so it reads a step's four pieces at once behind the step's one barrier; four LDS stages give
+// the loads three steps to arrive.  (4 pieces one after the other: 64 x 4096 x 4096 13.3 us instead of 12.8; two stages: weights out of
+// HBM, 128 x 8192 x 8192, 33.7 us instead of 22.0.)
 template <int T, int BM, int BN, int WM, int WN, int NST, bool DMA>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(const LinearArgs a) {
-    constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN;
-    constexpr int MT = WM / 32, NT = WN / 32;
-    constexpr int STAGE = (BM + BN) * 128;
-    constexpr int JA = BM * 8 / NTHR, J = (BM + BN) * 8 / NTHR;  // 16-byte pieces per thread and step: of x, in all
-    constexpr int PITCH = WN + 4;                                // epilogue image of a wave: 32 rows of WN sums
-    constexpr int EPI = NWM * NWN * 32 * PITCH * 4;
-    constexpr bool FLAT = MT * NT <= 2;
-    constexpr int NF = FLAT ? 4 : 2;  // pieces held in registers
-    static_assert(BM * 8 % NTHR == 0 && BN * 8 % NTHR == 0 && NTHR / 8 % 16 == 0 && (NST == 2 || NST == 4), "");
-    __shared__ __attribute__((aligned(16))) uint8_t s_mem[(NST * STAGE > EPI ? NST * STAGE : EPI)];
+    constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN, MT = WM / 32, NT = WN / 32;
+    constexpr int EPI = NWM * NWN * 32 * (WN + 4) * 4;
+    typedef Loader<T, BM, BN, NTHR, NST, false> L;
+    constexpr int J = L::J;
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[(NST * L::STAGE > EPI ? NST * L::STAGE : EPI)];
     __shared__ int s_xrow[BM], s_yrow[BM];
     __shared__ float s_scale[T == I8 ? BM : 1];
     const Tile t = find_tile<BM, 4>(a);
@@ -362,155 +429,62 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     rows_to_lds<T, BM, NTHR>(a, t, tid, s_xrow, s_yrow, s_scale);
     __syncthreads();
-    const int lc = ((tid & 7) ^ ((tid >> 4) & 7)) * 16;  // the 16-byte piece this thread moves in every row it touches
-    const int c_base = t.nt * BN;
-    const uint8_t *pp[J];  // its rows: JA of x, the others of w
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const int row = ((tid + j * NTHR) >> 3);
-        pp[j] = (j < JA ? a.x + (long)max(s_xrow[j < JA ? row : 0], 0) * a.ldx : a.w + ((long)t.g * a.n + min(c_base + row - BM, a.n - 1)) * a.ldw) + lc;
-    }
-    const int full = a.kb >> 7, steps = (a.kb + 127) >> 7;
-    auto stage = [&](int i) { return s_mem + (i & (NST - 1)) * STAGE; };
-    auto dma = [&](int i, int j) {
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(pp[j] + (long)i * 128),
-                                         (__attribute__((address_space(3))) void *)(stage(i) + wave * 1024 + j * NTHR * 16), 16, 0, 0);
-    };
-    auto copy_tail = [&](int i) {  // the partial step behind the full ones
-#pragma unroll
-        for (int j0 = 0; j0 < J; j0 += 4) {  // four loads on their way at a time
-            u32x4 v[4];
-#pragma unroll
-            for (int j = 0; j < 4 && j0 + j < J; ++j) v[j] = load16_tail(pp[j0 + j] - lc, i * 128 + lc, a.kb);
-#pragma unroll
-            for (int j = 0; j < 4 && j0 + j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + (j0 + j) * NTHR) * 16) = v[j];
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    u32x4 regs[DMA ? 1 : J];
-    auto load_regs = [&](int i, u32x4 (&to)[DMA ? 1 : J]) {
-#pragma unroll
-        for (int j = 0; j < J; ++j) to[DMA ? 0 : j] = load16(pp[j] + (long)i * 128);
-    };
-    auto put_regs = [&](int i, const u32x4 (&from)[DMA ? 1 : J]) {
-#pragma unroll
-        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + j * NTHR) * 16) = from[DMA ? 0 : j];
-    };
-    const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 31, hi = lane >> 5;
-    constexpr bool EARLY = MT * NT < 8;  // registers for them: on their way under the product
-    Chan<T, 8> ch;
-    if constexpr (EARLY) ch.load(a, t.g, c_base + wn + (lane % (WN / 8)) * 8);
+    const L l(a, t, s_mem, s_xrow, tid, wave);
+    const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 31, hi = lane >> 5, c_wave = t.nt * BN + wn;
+    Chan<T, 8> ch;  // on their way under the product
+    ch.load(a, t.g, c_wave + (lane % (WN / 8)) * 8);
     typename Acc<T>::q16 acc[NT][MT] = {};
     const uint8_t *sa = s_mem + (wm + li) * 128, *sb = s_mem + (BM + wn + li) * 128;
-    u32x4 fa[NF][MT], fb[NF][NT];
     // MV: the 32-row pieces of this wave that hold rows -- a group's last tile is seldom full, and matrix instructions on nothing
     // would cost as much as others
-    auto read = [&](auto MV, int i, int ks, int to) {
-        const int c = (i & (NST - 1)) * STAGE + ((ks * 2 + hi) ^ ((li >> 1) & 7)) * 16;
-        if constexpr (MV.value > 0) {
+    auto product = [&](auto MV, int i) {
+        u32x4 fa[4][MT], fb[4][NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) fb[to][j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
-        }
+        for (int ks = 0; ks < 4; ++ks) {
+            const int c = (i & (NST - 1)) * L::STAGE + ((ks * 2 + hi) ^ ((li >> 1) & 7)) * 16;
+            if constexpr (MV.value > 0) {
 #pragma unroll
-        for (int m = 0; m < MV.value; ++m) fa[to][m] = *reinterpret_cast<const u32x4 *>(sa + m * 4096 + c);
-    };
-    // a piece; `send`: the loads of step i among its matrix instructions
-    auto multiply = [&](auto MV, int from, bool send, int i) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-#pragma unroll
-            for (int m = 0; m < MV.value; ++m) mma32<T>(acc[j][m], fb[from][j], fa[from][m]);
-            if constexpr (DMA) {
-                if (send) {
-#pragma unroll
-                    for (int l = j * J / NT; l < (j + 1) * J / NT; ++l) dma(i, l);
-                }
+                for (int j = 0; j < NT; ++j) fb[ks][j] = *reinterpret_cast<const u32x4 *>(sb + j * 4096 + c);
             }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // this wave's loads of step i are in LDS; those of younger steps may still be on their way
-    auto landed = [&](int i) {
-        const int younger = min(NST - 2, full - 1 - i);
-        if (NST > 3 && younger >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * J) : "memory");
-        else if (NST > 2 && younger == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(J) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    };
-    // the first steps: all stages, or (FLAT through registers) the first step, with the second one's loads on their way
-    constexpr int AHEAD = FLAT && !DMA ? 1 : NST;
-    for (int i = 0; i < AHEAD; ++i) {
-        if (i < full) {
-            if constexpr (DMA) {
 #pragma unroll
-                for (int j = 0; j < J; ++j) dma(i, j);
-            } else {
-                load_regs(i, regs);
-                put_regs(i, regs);
-            }
-        } else if (i < steps) copy_tail(i);
-    }
-    if constexpr (FLAT && !DMA) {
-        if (1 < full) load_regs(1, regs);
-    }
-    auto barrier = [&] {  // this wave's LDS reads have come back, its LDS writes are done
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            for (int m = 0; m < MV.value; ++m) fa[ks][m] = *reinterpret_cast<const u32x4 *>(sa + m * 4096 + c);
+        }
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int m = 0; m < MV.value; ++m) mma32<T>(acc[j][m], fb[ks][j], fa[ks][m]);
         __builtin_amdgcn_sched_barrier(0);
     };
+    l.first(DMA ? NST : 1, DMA);
     auto walk = [&](auto MV) {
-        if constexpr (FLAT && DMA) {
-            for (int i = 0; i < steps; ++i) {
-                landed(i);
-                barrier();  // step i is in LDS, everyone has read step i - 1
+        if constexpr (DMA) {
+            for (int i = 0; i < l.steps; ++i) {
+                l.landed(i);
+                L::barrier();  // step i is in LDS, everyone has read step i - 1
                 const int next = i - 1 + NST;
-                if (i > 0 && next < full) {
+                if (i > 0 && next < l.full) {
 #pragma unroll
-                    for (int j = 0; j < J; ++j) dma(next, j);
-                } else if (i > 0 && next == full && full < steps) copy_tail(full);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) read(MV, i, ks, ks);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) multiply(MV, ks, false, 0);
-            }
-        } else if constexpr (FLAT) {
-            // step i + 2's registers are loaded while step i is multiplied, step i + 1's go to LDS behind it
-            auto half = [&](int i, u32x4 (&now)[DMA ? 1 : J], u32x4 (&later)[DMA ? 1 : J]) {
-                barrier();  // step i is in LDS, everyone has read step i - 1
-                if (i + 2 < full) load_regs(i + 2, later);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) read(MV, i, ks, ks);
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) multiply(MV, ks, false, 0);
-                if (i + 1 < full) put_regs(i + 1, now);
-                else if (i + 1 == full && full < steps) copy_tail(full);
-            };
-            u32x4 other[DMA ? 1 : J];
-            for (int i = 0; i < steps; i += 2) {
-                half(i, regs, other);
-                if (i + 1 < steps) half(i + 1, other, regs);
+                    for (int j = 0; j < J; ++j) l.dma(next, j);
+                } else if (i > 0 && next == l.full && l.full < l.steps) l.tail(l.full);
+                product(MV, i);
             }
         } else {
-            landed(0);
-            barrier();
-            if (steps > 0) read(MV, 0, 0, 0);
-            for (int i = 0; i < steps; ++i) {
-                const bool more = !DMA && i > 0 && i + NST - 1 < full;
-                if (more) load_regs(i + NST - 1, regs);
-                read(MV, i, 1, 1);
-                multiply(MV, 0, false, 0);
-                read(MV, i, 2, 0);
-                multiply(MV, 1, false, 0);
-                read(MV, i, 3, 1);
-                multiply(MV, 0, false, 0);
-                if (more) put_regs(i + NST - 1, regs);
-                landed(i + 1);
-                barrier();  // the last piece's fragments are in registers everywhere, step i + 1 is in LDS
-                if (i + NST == full && full < steps) copy_tail(full);
-                if (i + 1 < steps) read(MV, i + 1, 0, 0);
-                multiply(MV, 1, DMA && i + NST < full, i + NST);
+            // step i + 2's registers are loaded while step i is multiplied, step i + 1's go to LDS behind it
+            u32x4 even[J], odd[J];
+            if (1 < l.full) l.load(1, even);
+            auto half = [&](int i, const u32x4 (&now)[J], u32x4 (&later)[J]) {
+                L::barrier();  // step i is in LDS, everyone has read step i - 1
+                if (i + 2 < l.full) l.load(i + 2, later);
+                product(MV, i);
+                if (i + 1 < l.full) l.put(i + 1, now);
+                else if (i + 1 == l.full && l.full < l.steps) l.tail(l.full);
+            };
+            for (int i = 0; i < l.steps; i += 2) {
+                half(i, even, odd);
+                if (i + 1 < l.steps) half(i + 1, odd, even);
             }
         }
     };
@@ -518,9 +492,129 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
     if (valid <= 0) walk(std::integral_constant<int, 0>{});
     else if (MT > 1 && valid <= WM / 2) walk(std::integral_constant<int, (MT > 1 ? MT / 2 : MT)>{});
     else walk(std::integral_constant<int, MT>{});
-    if constexpr (!EARLY) ch.load(a, t.g, c_base + wn + (lane % (WN / 8)) * 8);
     __syncthreads();  // the stages become the waves' epilogue images
-    store_tile<T, MT, NT, WN>(a, ch, acc, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_base + wn, valid);
+    // 32 x 32 sums: lane l has row l % 32, channels 8 q + 4 (l / 32) + 0 .. 3
+    auto image = [&](auto *img, int i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<typename Acc<T>::q4 *>(img + li * (WN + 4) + j * 32 + q * 8 + hi * 4) =
+                    typename Acc<T>::q4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+    };
+    store_tile<T, MT, WN>(a, ch, image, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_wave, valid);
+}
+
+// ---- k_linear_wide: large tiles -- 256 x 256 with waves of 128 x 64, 128 x 128 with waves of 64 x 64 -------------------------------------------
+// For products that fill the chip with such tiles.  16 x 16 matrix instructions: they read and write their sums half as often per
+// multiplication as the 32 x 32 ones, and what limits these products is power (8192^3, clocks fall to 1.75 GHz on random data, the same
+// kernel runs a third faster on zeros): i8 423 us instead of 475, f16 794 instead of 892, bf16 745 instead of 846.
+// A step is 2 MT slots, one 16-row fragment of x each (MT pieces of the first 64 bytes, then of the second) against the wave's NT
+// channel fragments.  Fragments of x are read PF slots ahead into a ring of PF + 1, the channels' a half step ahead.  The one
+// barrier of a step stands PF slots before its end, where all that is left of the step is in registers: behind it the step's stage is
+// free, so the loads of step i + NST leave there, among the matrix instructions, and have NST - 1 steps to arrive, and the first
+// fragments of step i + 1 are read -- the matrix pipe has work across the barrier.  A partial step comes behind them, by itself.
+template <int T, int BM, int BN, int WM, int WN, int NST, int PF, bool DMA>
+__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_wide(const LinearArgs a) {
+    constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN, MT = WM / 16, NT = WN / 16, SLOTS = 2 * MT, X = SLOTS - PF;
+    constexpr int EPI = NWM * NWN * 32 * (WN + 4) * 4;
+    typedef Loader<T, BM, BN, NTHR, NST, true> L;
+    constexpr int J = L::J;
+    static_assert(SLOTS % (PF + 1) == 0 && X >= MT && NT <= MT && PF >= 1, "");
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[(NST * L::STAGE > EPI ? NST * L::STAGE : EPI)];
+    __shared__ int s_xrow[BM], s_yrow[BM];
+    __shared__ float s_scale[T == I8 ? BM : 1];
+    const Tile t = find_tile<BM, 4>(a);
+    if (t.r0 >= t.r1) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    rows_to_lds<T, BM, NTHR>(a, t, tid, s_xrow, s_yrow, s_scale);
+    __syncthreads();
+    const L l(a, t, s_mem, s_xrow, tid, wave);
+    const int wm = wave / NWN * WM, wn = wave % NWN * WN, li = lane & 15, q = lane >> 4, c_wave = t.nt * BN + wn;
+    typename Acc<T>::q4 acc[NT][MT] = {};
+    const uint8_t *sa = s_mem + (wm + li) * 128, *sb = s_mem + (BM + wn + li) * 128;
+    const int piece[2] = {(q ^ (li & 7)) * 16, ((4 + q) ^ (li & 7)) * 16};
+    u32x4 fa[PF + 1], fb[2][NT];
+    auto read_x = [&](int i, int f) { fa[f % (PF + 1)] = *reinterpret_cast<const u32x4 *>(sa + (i & (NST - 1)) * L::STAGE + (f % MT) * 2048 + piece[f / MT]); };
+    auto read_w = [&](int i, int half, int j) { fb[half][j] = *reinterpret_cast<const u32x4 *>(sb + (i & (NST - 1)) * L::STAGE + j * 2048 + piece[half]); };
+    const int valid = t.r1 - t.r0 - wm;           // rows of this wave's part, and the 16-row fragments that hold some: a group's last
+    const int pieces = (max(valid, 0) + 15) / 16;  // tile is seldom full, and matrix instructions on nothing would cost as much as others
+    u32x4 regs[DMA ? 1 : J];
+    l.first(min(NST, l.full), DMA);
+    l.landed(0);
+    L::barrier();
+    if (l.full > 0) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) read_w(0, 0, j);
+#pragma unroll
+        for (int f = 0; f < PF; ++f) read_x(0, f);
+    }
+    auto walk = [&](auto ALL) {
+        for (int i = 0; i < l.full; ++i) {
+#pragma unroll
+            for (int f = 0; f < SLOTS; ++f) {
+                if (f + PF < SLOTS) read_x(i, f + PF);
+                if (f < NT) read_w(i, 1, f);
+                if (f == X) {
+                    if constexpr (!DMA) {
+                        if (i > 0 && i - 1 + NST < l.full) l.put(i - 1 + NST, regs);
+                    }
+                    l.landed(i + 1);
+                    L::barrier();  // the rest of step i is in registers everywhere, step i + 1 is in LDS
+                    if constexpr (!DMA) {
+                        if (i + NST < l.full) l.load(i + NST, regs);
+                    }
+                    if (i + 1 < l.full) {
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) read_w(i + 1, 0, j);
+                    }
+                }
+                if (f >= X && i + 1 < l.full) read_x(i + 1, f - X);
+                if (ALL.value || f % MT < pieces) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma16<T>(acc[j][f % MT], fb[f / MT][j], fa[f % (PF + 1)]);
+                }
+                if constexpr (DMA) {
+                    constexpr int PER = (J + PF - 1) / PF;
+                    if (f >= X && i + NST < l.full) {
+#pragma unroll
+                        for (int j = (f - X) * PER; j < (f - X + 1) * PER && j < J; ++j) l.dma(i + NST, j);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    if (pieces >= MT) walk(std::true_type{});  // a branch at every slot costs 7 %
+    else walk(std::false_type{});
+    if (l.full < l.steps) {  // the partial step, by itself
+        L::barrier();
+        l.tail(l.full);
+        L::barrier();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) read_w(l.full, h, j);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                read_x(l.full, h * MT + m);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) mma16<T>(acc[j][m], fb[h][j], fa[(h * MT + m) % (PF + 1)]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    Chan<T, 8> ch;
+    ch.load(a, t.g, c_wave + (lane % (WN / 8)) * 8);
+    __syncthreads();  // the stages become the waves' epilogue images
+    // 16 x 16 sums: lane l has row l % 16, channels 4 (l / 16) + 0 .. 3
+    auto image = [&](auto *img, int i) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *reinterpret_cast<typename Acc<T>::q4 *>(img + (h * 16 + li) * (WN + 4) + j * 16 + q * 4) = acc[j][2 * i + h];
+    };
+    store_tile<T, WM / 32, WN>(a, ch, image, s_mem, s_yrow + wm, s_scale + (T == I8 ? wm : 0), wave, lane, c_wave, valid);
 }
 
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
