@@ -42,43 +42,55 @@ bool misaligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(si
 
 constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 stays far inside 64 bits
 
-// The forms of a product.  What a launch costs goes, to within a tenth or two, as 3 us + the number of rounds of workgroups it takes
-// times a form's own time per round and summed byte, whatever the type's size -- measured on dense products of 4096 channels by
-// 4096 bytes of K, us for (rounds of) workgroups:
-//   few 16 x 16   256: 6.4  512: 10.4  1024: 17.8        tile 64    256: 12.9  512: 19.2  1024: 34.6  2048: 68.0
-//   few 32 x 16   256: 8.3  512: 13.7  1024: 25.1        tile 128   256: 26.4 (4 stages, one workgroup per CU)  512: 51.3
-//   few 32 x 32   256: 10.4 512: 17.6  1024: 31.7        tile 128w  256: 31.7 (2 stages, two per CU)  512: 43.4
-//                                                        tile 256   256: 56 .. 61
-// A tile that holds next to no rows costs the few forms less (`thin`; 1 x 4096: 5.1 against 6.4; 32 rows over 64 groups, 2048 x 2048
-// bf16: 16 x 16 32 us, 32 x 32 50, tile 64 42).  f32 runs at the f32 matrix rate, a sixteenth of the others': larger tiles gain less there.  Rows off 16 bytes cost the
-// few forms twice and more (16 x 4096 x 4099: 14.1 us, tile 64 18.6; 64 rows: 24.3, 21.6), the tiles a third to a half.  The form with
-// the least such cost is taken; sums of 8-bit products are the same by every form.
-enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, TILE128W, TILE256, FORMS };
+// The forms of a product.  A launch is taken to cost a start-up time, plus the number of rounds of workgroups it takes times (a form's
+// own fixed time + its time per 4096 summed bytes), whatever the type's size, or the time of its bytes at the copy rate if that is more.
+// Dense products, us:
+//                 4096 channels by 4096 bytes of K, so many workgroups        4330 x 7218 by 64   4096 x 4096 by 4096 bytes, rows
+//                 (rows on 16 bytes)                                          bytes               on 16 bytes    on 4   odd
+//   few 16 x 16   256: 6.4   512: 10.4  1024: 17.8                            441                 909           1076   1566
+//   few 32 x 16   256: 8.3   512: 13.7  1024: 25.1                            404                 720            832   1304
+//   few 32 x 32   256: 10.4  512: 17.6  1024: 31.7                            127                 454            499    726
+//   tile 64       256: 12.9  512: 19.2  1024: 34.6  2048: 68.0                 86                 132            171    205
+//   tile 128      256: 26.4  512: 51.3 (one workgroup per CU)                  66                  94            127    158
+//   wide 128      256: 30.5  512: 40.6  1024: 76.5 (two per CU)                57                  83             94    125
+//   wide 256      128: 55    256: 60    512: 123                               52                  62             88     98
+// A tile that holds next to no rows costs less (`thin`: its loads of x are of one row); f32 runs at the f32 matrix rate, a sixteenth of
+// the others', and larger tiles gain less there; a longer program starts later when it is not in the instruction caches.  The figures
+// below start from these and are fitted to the times of all seven forms on 1320 products, dense and grouped, of all types and
+// alignments, 1 to 16384 rows, 32 to 8192 channels and values, launched back to back and after other work: the form with the least such
+// cost, which is taken, ran 2.4 and 1.2 % longer than the best one there in the geometric mean.  Sums of 8-bit products are the same by
+// every form.
+enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, WIDE128, WIDE256, FORMS };
 struct FormCost {
     int bm, bn, slots;  // tile, workgroups per round
-    float cost, cost_f32, cost_off, thin;
+    float start, fixed, cost, cost4, cost_odd, cost_f32, thin;  // costs: rows on 16 bytes, on 4, on less; f32 rows
 };
-constexpr FormCost FORM[FORMS] = {{16, 16, 256, 3.7f, 3.7f, 11.f, 0.48f},  {32, 16, 256, 5.5f, 5.4f, 16.f, 0.8f}, {32, 32, 256, 7.4f, 8.5f, 20.5f, 0.8f},
-                                  {64, 64, 256, 8.6f, 19.5f, 15.f, 1.f},   {128, 128, 256, 24.f, 65.f, 41.f, 1.f}, {128, 128, 512, 40.f, 127.f, 60.f, 1.f},
-                                  {256, 256, 256, 56.f, 1e9f, 92.f, 1.f}};
+constexpr FormCost FORM[FORMS] = {
+    {16, 16, 256, 5.8f, 1.1f, 3.0f, 1.9f, 3.8f, 3.0f, 0.66f},   {32, 16, 256, 6.0f, 0.9f, 3.9f, 4.6f, 4.3f, 5.5f, 1.f},     {32, 32, 256, 6.0f, 1.0f, 5.5f, 6.8f, 6.0f, 7.2f, 1.f},
+    {64, 64, 256, 6.7f, 1.9f, 9.2f, 16.f, 13.6f, 17.5f, 0.68f}, {128, 128, 256, 6.8f, 7.1f, 18.6f, 46.f, 40.f, 64.f, 0.59f}, {128, 128, 512, 8.9f, 8.3f, 28.f, 41.f, 41.f, 122.f, 0.77f},
+    {256, 256, 256, 10.2f, 15.f, 31.6f, 86.f, 84.f, 1e9f, 0.74f}};
 
-// row tiles of bm rows: what the groups can have at most (every group but one may end inside a tile) ...
+// what the groups' rows can take in tiles of bm rows at most (every group but one may end inside a tile) ...
 long most_row_tiles(const LinearArgs &a, long bm) {
     return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm;
 }
 
-Form pick_form(const LinearArgs &a, bool f32, bool aligned) {
-    // ... and will have: the lengths are not known here, a group's last tile is half full in the middle (512 rows over 8 groups of 40
-    // to 110, 256 x 1280 f32: taken as 8 x 2 full tiles of 32 rows the product took 20 us by 32 x 16, by 32 x 32 15)
-    const float groups = (float)std::min(a.groups, a.m), rows = (float)a.m / groups;
+Form pick_form(const LinearArgs &a, bool f32, int align) {
+    // ... and will take: the lengths are not known here.  So many groups have rows if the rows fall evenly; a group's last tile is half
+    // full in the middle, and so is the last round
+    const bool many = a.offsets && a.groups > 1;
+    const float groups = many ? a.groups * (1.f - std::exp(-(float)a.m / a.groups)) : 1.f, rows = (float)a.m / groups;
+    const float bytes = ((groups * a.n + a.m) * (float)a.kb + 2.f * a.m * a.n) / 5.1e6f;
     int best = FEW11;
     float least = 3.4e38f;
     for (int i = 0; i < FORMS; ++i) {
         const FormCost &f = FORM[i];
-        const float per_group = groups > 1 ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)((a.m + f.bm - 1) / f.bm);
-        const float tiles = groups * per_group * (float)((a.n + f.bn - 1) / f.bn);
-        float c = std::ceil(tiles / (float)f.slots) * std::max(f32 ? f.cost_f32 : f.cost, aligned ? 0.f : f.cost_off);
-        c *= f.thin + (1.f - f.thin) * std::min(1.f, rows / (float)f.bm);
+        const float per_group = many ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)((a.m + f.bm - 1) / f.bm);
+        const float all = groups * per_group * (float)((a.n + f.bn - 1) / f.bn) / (float)f.slots;
+        const float rounds = many ? std::max(1.f, all + 0.5f) : std::ceil(all);
+        const float thin = f.thin + (1.f - f.thin) * std::min(1.f, rows / (float)f.bm);
+        const float cost = f32 ? f.cost_f32 : align == 16 ? f.cost : align == 4 ? f.cost4 : f.cost_odd;
+        const float c = f.start + std::max(bytes, rounds * thin * (f.fixed + cost * (float)a.kb / 4096.f));
         if (c < least) {
             least = c;
             best = i;
@@ -87,22 +99,24 @@ Form pick_form(const LinearArgs &a, bool f32, bool aligned) {
     return (Form)best;
 }
 
-template <int T, bool ALIGNED>
+// AL: every row of x and w starts on so many bytes (16: loads straight into LDS; 4; less)
+template <int T, int AL>
 int launch(LinearArgs a, hipStream_t s) {
-    const Form f = pick_form(a, T == F32, ALIGNED);
+    const Form f = pick_form(a, T == F32, AL);
     const long row_tiles = most_row_tiles(a, FORM[f].bm), n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
     PB_CHECK(row_tiles < (INT_MAX - 8) / n_tiles, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
     a.n_tiles = (int)n_tiles;
     const dim3 grid((unsigned)((row_tiles * n_tiles + 7) / 8 * 8));
+    constexpr bool DW = AL >= 4;
     switch (f) {
-        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4>), grid, dim3(512), 0, s, a); break;
-        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4>), grid, dim3(512), 0, s, a); break;
-        case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2>), grid, dim3(512), 0, s, a); break;
-        case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, ALIGNED ? 4 : 2, ALIGNED>), grid, dim3(256), 0, s, a); break;
-        case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, ALIGNED>), grid, dim3(512), 0, s, a); break;
-        case TILE128W: hipLaunchKernelGGL((k_linear_wide<T, 128, 128, 64, 64, 2, 3, ALIGNED>), grid, dim3(256), 0, s, a); break;
+        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, DW>), grid, dim3(512), 0, s, a); break;
+        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4, DW>), grid, dim3(512), 0, s, a); break;
+        case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2, DW>), grid, dim3(512), 0, s, a); break;
+        case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, AL == 16 ? 4 : 2, AL == 16>), grid, dim3(256), 0, s, a); break;
+        case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, AL == 16>), grid, dim3(512), 0, s, a); break;
+        case WIDE128: hipLaunchKernelGGL((k_linear_wide<T, 128, 128, 64, 64, 2, 3, AL == 16>), grid, dim3(256), 0, s, a); break;
         default:
-            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_wide<T, 256, 256, 128, 64, 2, ALIGNED ? 7 : 1, ALIGNED>), grid, dim3(512), 0, s, a);
+            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_wide<T, 256, 256, 128, 64, 2, AL == 16 ? 7 : 1, AL == 16>), grid, dim3(512), 0, s, a);
             break;
     }
     PB_HIP(hipGetLastError());
@@ -110,8 +124,12 @@ int launch(LinearArgs a, hipStream_t s) {
 }
 template <int T>
 int launch(const LinearArgs &a, hipStream_t s) {
-    const bool aligned = !misaligned(a.x, 16) && !misaligned(a.w, 16) && a.ldx % 16 == 0 && a.ldw % 16 == 0;
-    return aligned ? launch<T, true>(a, s) : launch<T, false>(a, s);
+    const uint64_t low = (uint64_t)(uintptr_t)a.x | (uint64_t)(uintptr_t)a.w | (uint64_t)a.ldx | (uint64_t)a.ldw;
+    if (low % 16 == 0) return launch<T, 16>(a, s);
+    if constexpr (T != F32) {
+        if (low % 4 != 0) return launch<T, 1>(a, s);
+    }
+    return launch<T, 4>(a, s);
 }
 
 // what pb_linear_i8 and pb_linear_grouped have in common

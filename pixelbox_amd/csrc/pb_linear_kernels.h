@@ -65,19 +65,34 @@ __device__ __forceinline__ void mma32(typename Acc<T>::q16 &c, const u32x4 &a, c
 }
 
 // ---- loads and stores of any alignment ---------------------------------------------------------------------------------------------------
-// global_load / store_dwordx4 take any address; aligned ones are not slower for it.
+// global_load / store_dwordx4 take any address; what that costs depends on the bound.  Tiles load a byte once for many products: on
+// 4 bytes or less they lose up to the difference between DMA and registers (4096^3 i8 by 256 x 256: 62 us aligned, 88 on 4 bytes, 98
+// odd).  The few forms live on loads, which go at full rate on 4 bytes and at a third off them (41 x 217 x 3903 f16: 26.6 us, with
+// 3904 values 10.1): there (DW false) the aligned words around the 16 bytes are read -- only such as hold at least one of them -- and
+// shifted into place (13.0 us; in tiles that costs more than it saves: 777 x 1003 x 1289 i8 12.6 us, plain 11.2).
+template <bool DW>
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) {
     u32x4 v;
-    __builtin_memcpy(&v, p, 16);
-    return v;
+    if constexpr (DW) {
+        __builtin_memcpy(&v, p, 16);
+        return v;
+    } else {
+        const uint32_t sh = (uint32_t)(uintptr_t)p & 3u;
+        const uint8_t *d = p - sh;
+        __builtin_memcpy(&v, __builtin_assume_aligned(d, 4), 16);
+        const uint32_t e = *reinterpret_cast<const uint32_t *>(d + (sh ? 16 : 12));
+        return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, sh), __builtin_amdgcn_alignbyte(v.z, v.y, sh), __builtin_amdgcn_alignbyte(v.w, v.z, sh),
+                     __builtin_amdgcn_alignbyte(e, v.w, sh)};
+    }
 }
 __device__ __forceinline__ void store16(uint8_t *p, const u32x4 &v) { __builtin_memcpy(p, &v, 16); }
 // bytes [at, at + 16) of a row of `len` bytes, zero behind its end; reads nothing outside [0, len).  Without a branch for rows of 16
 // bytes and more, so that several such loads are on their way together: the row's last 16 bytes, shifted down.
+template <bool DW>
 __device__ __forceinline__ u32x4 load16_tail(const uint8_t *row, int at, int len) {
     if (len >= 16) {
         const int off = min(at, len - 16), s = 8 * (at - off);
-        const u32x4 t = load16(row + off);
+        const u32x4 t = load16<DW>(row + off);
         const uint64_t lo = ((uint64_t)t.y << 32) | t.x, hi = ((uint64_t)t.w << 32) | t.z;
         const uint64_t l2 = s == 0 ? lo : s < 64 ? (lo >> s) | (hi << (64 - s)) : s < 128 ? hi >> (s - 64) : 0;
         const uint64_t h2 = s < 64 ? hi >> s : 0;
@@ -189,9 +204,22 @@ __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
 }
 
 // ---- epilogue: scales, bias, activation, one rounding, store ------------------------------------------------------------------------------
+// tanh x = (1 - e^-2|x|) / (1 + e^-2|x|) with x's sign; below 0.4, where the difference loses digits, its series to x^11 (the next
+// term is 6e-8 of the sum there).  Within 9 units of 2^-24 (at 0.4: the exponential is off by (2 |x| + 2) units, which the numerator
+// magnifies by e / (1 - e) = 0.82; its own rounding, the denominator's, the reciprocal's two and the product's).  The library's tanhf
+// (2 units in the last place) took 26 of the 63 us of 4330 x 7218 x 64.
+__device__ __forceinline__ float tanh_f(float x) {
+    const float a = fabsf(x), e = __builtin_amdgcn_exp2f(a * -2.8853900817779268f);
+    const float far = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), z = x * x;
+    float p = __builtin_fmaf(z, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    p = __builtin_fmaf(z, p, -17.0f / 315.0f);
+    p = __builtin_fmaf(z, p, 2.0f / 15.0f);
+    p = __builtin_fmaf(z, p, -1.0f / 3.0f);
+    return a < 0.4f ? __builtin_fmaf(x * z, p, x) : copysignf(far, x);
+}
 __device__ __forceinline__ float act_f(float v, int act) {
     if (act == PB_ACT_SILU) return pbe::silu_f(v);
-    if (act == PB_ACT_TANH) return tanhf(v);
+    if (act == PB_ACT_TANH) return tanh_f(v);
     return v;
 }
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -331,8 +359,8 @@ __device__ __forceinline__ void store_tile(const LinearArgs &a, const Chan<T, 8>
 // eight 16-byte pieces permuted, so that the fragment reads -- 16 bytes from each of 32 (or of 16 x 4) places -- are free of bank
 // conflicts: with 32-row fragments piece c at c ^ (row / 2 & 7): 249 bytes a clock and CU, against 121 with c ^ (row & 7) and 32
 // unpermuted; with 16-row fragments c ^ (row & 7): 242 (LDS reads alone, 256 workgroups of eight waves).  The permutation is done by
-// the lanes' GLOBAL addresses, so a wave's eight rows of 128 bytes are still whole lines.  DMA: the loads go straight into LDS
-// (16-byte aligned rows); otherwise through registers, which takes any alignment.  The last, partial step always goes through registers.
+// the lanes' GLOBAL addresses, so a wave's eight rows of 128 bytes are still whole lines.  DMA: the
+// loads go straight into LDS (16-byte aligned rows); otherwise through registers, which takes any alignment.  The last, partial step always goes through registers.
 template <int T, int BM, int BN, int NTHR, int NST, bool ROWS16>
 struct Loader {
     static constexpr int TAIL = BM > 128 ? 2 : 4;
@@ -363,7 +391,7 @@ struct Loader {
     }
     __device__ __forceinline__ void load(int i, u32x4 (&to)[J]) const {
 #pragma unroll
-        for (int j = 0; j < J; ++j) to[j] = load16(pp[j] + (long)i * 128);
+        for (int j = 0; j < J; ++j) to[j] = load16<true>(pp[j] + (long)i * 128);
     }
     __device__ __forceinline__ void put(int i, const u32x4 (&from)[J]) const {
 #pragma unroll
@@ -374,7 +402,7 @@ struct Loader {
         for (int j0 = 0; j0 < J; j0 += TAIL) {  // a few loads on their way at a time
             u32x4 v[TAIL];
 #pragma unroll
-            for (int j = 0; j < TAIL && j0 + j < J; ++j) v[j] = load16_tail(pp[j0 + j] - lc, i * 128 + lc, kb);
+            for (int j = 0; j < TAIL && j0 + j < J; ++j) v[j] = load16_tail<true>(pp[j0 + j] - lc, i * 128 + lc, kb);
 #pragma unroll
             for (int j = 0; j < TAIL && j0 + j < J; ++j) *reinterpret_cast<u32x4 *>(stage(i) + (tid + (j0 + j) * NTHR) * 16) = v[j];
             __builtin_amdgcn_sched_barrier(0);
@@ -620,7 +648,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_wide(cons
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
 // For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
 // waves' partial sums meet in LDS and are added in wave order.
-template <int T, int MT, int NT, int NW, int U>
+template <int T, int MT, int NT, int NW, int U, bool DW>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     typedef typename Acc<T>::e E;
     typedef typename Acc<T>::q4 Q;
@@ -645,17 +673,30 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16(pw[j] + kb + u * 64);
+                for (int j = 0; j < NT; ++j) fw[u][j] = load16<DW>(pw[j] + kb + u * 64);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16(px[i] + kb + u * 64);
+                for (int i = 0; i < MT; ++i) fx[u][i] = load16<DW>(px[i] + kb + u * 64);
             }
         } else {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
+                const int at = kb + u * 64;
+                if (at + 64 <= kb1) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail(pw[j] - kq, kb + u * 64 + kq, kb1);
+                    for (int j = 0; j < NT; ++j) fw[u][j] = load16<DW>(pw[j] + at);
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail(px[i] - kq, kb + u * 64 + kq, kb1);
+                    for (int i = 0; i < MT; ++i) fx[u][i] = load16<DW>(px[i] + at);
+                } else if (at < kb1) {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) fw[u][j] = load16_tail<DW>(pw[j] - kq, at + kq, kb1);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) fx[u][i] = load16_tail<DW>(px[i] - kq, at + kq, kb1);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) fw[u][j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) fx[u][i] = u32x4{0, 0, 0, 0};
+                }
             }
         }
 #pragma unroll
@@ -753,7 +794,7 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
     const uint32_t INF = 0x7f800000u;
     auto load = [&](int c, float (&v)[V]) {
         if (c + V <= k) {
-            const u32x4 q = load16(px + (long)c * type_bytes(T));
+            const u32x4 q = load16<true>(px + (long)c * type_bytes(T));
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 if constexpr (T == F32) v[i] = __uint_as_float(q[i]);
@@ -820,7 +861,8 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
 // comparison into a lane mask: the counts come from the scalar unit's bit counts, the masks of matching rows go to LDS -- four
 // vector instructions for 64 rows, which is what bounds it (131072 rows, 256 groups: 27 us with a bit per lane put together by vector
 // instructions).  Then every thread takes a contiguous run of words of 32 rows, learns by a prefix sum over the bit counts where its
-// rows go, and writes them.  Rows beyond one LDS map's 8192 per wave are walked a second time, map by map.
+// rows go, and writes them.  Its stores go to lines apart, so the waves of a group that has a fifth of the rows or more write 64 rows'
+// worth side by side instead (131072 rows of one group: 74 us by threads, 21 by waves; of 8 groups: 15.6 and 20.8).  Rows beyond one LDS map's 8192 per wave are walked a second time, map by map.
 // As unsigned numbers, rows of no group are >= groups: a row is before group g if it is < g.
 // v with the wave-uniform `value` in one lane: v_writelane_b32 as the compiler's intrinsic, which has no builtin of its own (as inline
 // asm the compiler leaves out the two wait states between the comparison that writes the scalar register and this read of it)
@@ -899,38 +941,65 @@ __global__ __launch_bounds__(64 * WAVES, 8) void k_group_rows(const int32_t *__r
                 n = walk(LAST, c);
                 __syncthreads();
             }
-            const int words = (n + 31) >> 5, each = (words + NTHR - 1) / NTHR;  // 1 .. 4 words for a thread
+            const int words = (n + 31) >> 5, each = words <= NTHR ? 1 : words <= 2 * NTHR ? 2 : 4;  // for a thread
+            auto word = [&](int w) {  // lanes 8 (w % 8) .. + 8 of turn w / 8, a bit of each of the four masks in turn
+                const uint32_t *mask = s_mask + (w >> 3) * 8 + ((w >> 2) & 1);
+                uint32_t bits = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t x = (mask[2 * k] >> (8 * (w & 3))) & 255u;
+                    x = (x | x << 12) & 0x000f000fu;
+                    x = (x | x << 6) & 0x03030303u;
+                    x = (x | x << 3) & 0x11111111u;
+                    bits |= x << k;
+                }
+                return bits;
+            };
             uint32_t b[4];
             int count = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int w = tid * each + i;
-                b[i] = 0;
-                if (i < each && w < words) {  // word w: lanes 8 (w % 8) .. + 8 of turn w / 8, a bit of each of the four masks in turn
-                    const uint32_t *mask = s_mask + (w >> 3) * 8 + ((w >> 2) & 1);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t x = (mask[2 * k] >> (8 * (w & 3))) & 255u;
-                        x = (x | x << 12) & 0x000f000fu;
-                        x = (x | x << 6) & 0x03030303u;
-                        x = (x | x << 3) & 0x11111111u;
-                        b[i] |= x << k;
-                    }
-                }
+                b[i] = i < each && w < words ? word(w) : 0u;
                 count += __builtin_popcount(b[i]);
             }
             const int inc = wave_prefix(count);
             if (lane == 63) s_eq[wave] = inc;
             __syncthreads();
-            int to = first + inc - count;
+            int before = 0, all = 0;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                if (w < wave) to += s_eq[w];
-                first += s_eq[w];
+                if (w < wave) before += s_eq[w];
+                all += s_eq[w];
             }
+            if (5 * all < n) {  // every thread writes its own rows
+                int to = first + before + inc - count;
+                const int row0 = c * CHUNK + tid * each * 32;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                for (uint32_t left = b[i]; left; left &= left - 1) order[to++] = c * CHUNK + (tid * each + i) * 32 + __builtin_ctz(left);
+                for (int i = 0; i < 4; ++i)
+                    for (uint32_t left = b[i]; left; left &= left - 1) order[to++] = row0 + i * 32 + __builtin_ctz(left);
+            } else {  // a wave goes through its threads' words 64 rows at a time and writes these side by side
+                int to = first + before, row = c * CHUNK + wave * 64 * each * 32;
+                auto put = [&](int low, int high) {
+                    const uint64_t mine = (uint64_t)(uint32_t)high << 32 | (uint32_t)low;
+                    const int at = to + __builtin_amdgcn_mbcnt_hi((uint32_t)high, __builtin_amdgcn_mbcnt_lo((uint32_t)low, 0u));
+                    if (__builtin_amdgcn_inverse_ballot_w64(mine)) order[at] = row + lane;
+                    to += __builtin_popcountll(mine);
+                    row += 64;
+                };
+                auto of_lane = [](uint32_t v, int l) { return __builtin_amdgcn_readlane((int)v, l); };
+                if (each == 1) {
+#pragma unroll 4
+                    for (int l = 0; l < 64; l += 2) put(of_lane(b[0], l), of_lane(b[0], l + 1));
+                } else {
+#pragma unroll 4
+                    for (int l = 0; l < 64; ++l) {
+                        put(of_lane(b[0], l), of_lane(b[1], l));
+                        if (each == 4) put(of_lane(b[2], l), of_lane(b[3], l));
+                    }
+                }
+            }
+            first += all;
         }
     };
     if (g == (unsigned)groups) run(std::true_type{});
