@@ -276,7 +276,7 @@ int pb_embed_batch_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, uint
                           float *d_out_f32);
 
 /* The network up to its last layer: the pooled features (f32[n][1280], DEVICE, 16-byte aligned) that Linear(1280, D) + tanh make the
- * hash of (resources/train.py:30-46), for layers of the caller's own (the linear layers below).  n <= max_batch; stream
+ * hash of (resources/train.py:30-46), for layers of the caller's own (the linear layers below); not over the images.  n <= max_batch; stream
  * contract as pb_embed_batch_device. */
 int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, float *d_features);
 
@@ -285,7 +285,7 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
  * quantiser of efficientnet.rs:39, all on the embedder's stream (contract as pb_embed_batch_device).  All pointers are DEVICE memory.
  * type: PB_TYPE_F32 (d_w: f32[heads][d][1280]) or PB_TYPE_I8 (int8, with d_w_scale f32[heads][d]: pb_quantize_rows over the weights'
  * rows); d_bias: f32[heads][d] or NULL; d_head: int[n].  d_out_u8: uint8[n][d], d_out_f32: f32[n][d], either may be NULL.  Images
- * whose head is outside [0, heads) are left as they are in both.  The f32 product is summed in plain f32 (the embedder's own Linear
+ * whose head is outside [0, heads) are left as they are in both; the outputs overlap neither each other nor d_head.  The f32 product is summed in plain f32 (the embedder's own Linear
  * sums bf16 pieces): with the blob's own weights as the only head the values agree with pb_embed_batch to the embedding's tolerance,
  * not bit for bit.  An i8 head is off by the codes' rounding: half a code of 254 per feature and weight. */
 int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
@@ -416,8 +416,9 @@ int pb_phash_small_image(pb_phasher *p, const uint8_t *rgb, uint32_t width, uint
  *  A call checks its arguments, queues one kernel and returns: outputs are complete for later work on that stream, or once the
  *  caller has waited for it.  Nothing is allocated and no state outlives a call, so calls may run from any threads, on any streams,
  *  and inside a graph capture.  m = 0 (and n = 0) is a call that does nothing.
- *  ld* is the distance between rows in ELEMENTS; any value >= the row length, any alignment of a row to its type.  16-byte aligned
- *  rows run fastest.
+ *  ld* is the distance between rows in ELEMENTS; any value >= the row length, any alignment of a row to its type.  Rows on 16 bytes
+ *  run fastest, rows off 4 bytes (an odd k of 8- or 16-bit values without padding) slowest: about half as fast where the product
+ *  fills the GPU.  Rows number less than 2^31 - 256; no output may overlap an input or another output.
  * ====================================================================================== */
 #define PB_TYPE_F32 0
 #define PB_TYPE_BF16 1
@@ -454,7 +455,7 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
  * order of x; with only x_rows the groups' results lie packed, as the input of a next layer that has only y_rows.  offsets
  * (int[groups + 1]) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,
  * a row number outside x ([0, x_total)) or y ([0, y_total)) is skipped.  A row of x may be listed any number of times, a row of y
- * once (twice: either result stands).  Rows of y that are not listed are left as they are.  y must not overlap x or w. */
+ * once (twice: either result stands).  Rows of y that are not listed are left as they are. */
 int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
                       const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
                       void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k);

@@ -1961,6 +1961,9 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
     PB_CHECK(n <= e->max_batch, PB_ERR_INVALID, "pb_embed_features_device: n = %u > max_batch %u", n, e->max_batch);
     PB_CHECK(n == 0 || (d_rgb && d_features), PB_ERR_INVALID, "pb_embed_features_device: null buffer");
     PB_CHECK(((uintptr_t)d_features & 15) == 0, PB_ERR_INVALID, "pb_embed_features_device: d_features is not aligned to 16 bytes");
+    const uint64_t rgb_bytes = (uint64_t)n * e->H * e->W * 3, f_bytes = (uint64_t)n * 1280 * 4;
+    PB_CHECK((uintptr_t)d_features + f_bytes <= (uintptr_t)d_rgb || (uintptr_t)d_rgb + rgb_bytes <= (uintptr_t)d_features, PB_ERR_INVALID,
+             "pb_embed_features_device: d_features overlaps the images");
     if (n == 0) return PB_OK;
     std::lock_guard<std::mutex> lock(e->mu);
     pb::DeviceGuard guard(e->device);
@@ -1979,6 +1982,10 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
     PB_CHECK(d >= 1 && d <= (1u << 20), PB_ERR_INVALID, "pb_embed_heads_device: d = %u (1 .. 2^20)", d);
     PB_CHECK(n == 0 || (d_rgb && d_w && d_head && (d_out_u8 || d_out_f32) && (type != PB_TYPE_I8 || d_w_scale)), PB_ERR_INVALID,
              "pb_embed_heads_device: null buffer");
+    const auto apart = [](const void *p, uint64_t pb, const void *q, uint64_t qb) { return !p || !q || (uintptr_t)p + pb <= (uintptr_t)q || (uintptr_t)q + qb <= (uintptr_t)p; };
+    PB_CHECK(apart(d_out_u8, (uint64_t)n * d, d_out_f32, (uint64_t)n * d * 4) && apart(d_out_u8, (uint64_t)n * d, d_head, (uint64_t)n * 4) &&
+                 apart(d_out_f32, (uint64_t)n * d * 4, d_head, (uint64_t)n * 4),
+             PB_ERR_INVALID, "pb_embed_heads_device: outputs overlap each other or d_head");
     if (n == 0) return PB_OK;
     std::lock_guard<std::mutex> lock(e->mu);
     pb::DeviceGuard guard(e->device);
@@ -1993,16 +2000,10 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
     }
     float *val = d_out_f32;
     if (!val) {
-        if (e->hd_val_cap < B * d) {  // a wider head than any before: the smaller buffer goes once nothing queued uses it
-            if (e->hd_val) {
-                PB_HIP(hipStreamSynchronize(e->stream));
-                e->allocs.erase(std::find(e->allocs.begin(), e->allocs.end(), (void *)e->hd_val));
-                (void)hipFree(e->hd_val);
-                e->hd_val = nullptr;
-                e->hd_val_cap = 0;
-            }
-            if ((rc = dalloc(e, &e->hd_val, B * d))) return rc;
-            e->hd_val_cap = B * d;
+        if (e->hd_val_cap < B * d) {  // wider heads than any before; the smaller buffer stays, for what is queued or captured with it
+            const size_t cap = std::max(B * d, 2 * e->hd_val_cap);
+            if ((rc = dalloc(e, &e->hd_val, cap))) return rc;
+            e->hd_val_cap = cap;
         }
         val = e->hd_val;
     }

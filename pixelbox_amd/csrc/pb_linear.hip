@@ -40,7 +40,9 @@ uint64_t extent(uint64_t rows, uint64_t ld, uint64_t n, int size) { return rows 
 bool bad_type(int t) { return t != PB_TYPE_F32 && t != PB_TYPE_BF16 && t != PB_TYPE_F16; }
 bool misaligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(size - 1)) != 0; }
 
-constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 stays far inside 64 bits
+constexpr uint64_t MAX_LD = 1ull << 40, MAX_ROWS = INT_MAX - 256;  // a tile's end stays an int
+// rows at a stride of ld elements: row * ld * 4 stays far inside 64 bits
+bool fits(uint64_t rows, uint64_t ld) { return rows <= 1 || ld <= (1ull << 50) / rows; }
 
 // The forms of a product.  A launch is taken to cost a start-up time, plus the number of rounds of workgroups it takes times (a form's
 // own fixed time + its time per 4096 summed bytes), whatever the type's size, or the time of its bytes at the copy rate if that is more.
@@ -53,39 +55,43 @@ constexpr uint64_t MAX_LD = 1ull << 40;  // elements between rows: row * ld * 4 
 //   tile 64       256: 12.9  512: 19.2  1024: 34.6  2048: 68.0                 86                 132            171    205
 //   tile 128      256: 26.4  512: 51.3 (one workgroup per CU)                  66                  94            127    158
 //   wide 128      256: 30.5  512: 40.6  1024: 76.5 (two per CU)                57                  83             94    125
-//   wide 256      128: 55    256: 60    512: 123                               52                  62             88     98
+//   wide 256      128: 55    256: 60    512: 123                               52                  62
 // A tile that holds next to no rows costs less (`thin`: its loads of x are of one row); f32 runs at the f32 matrix rate, a sixteenth of
 // the others', and larger tiles gain less there; a longer program starts later when it is not in the instruction caches.  The figures
-// below start from these and are fitted to the times of all seven forms on 1320 products, dense and grouped, of all types and
-// alignments, 1 to 16384 rows, 32 to 8192 channels and values, launched back to back and after other work: the form with the least such
-// cost, which is taken, ran 2.4 and 1.2 % longer than the best one there in the geometric mean.  Sums of 8-bit products are the same by
+// below start from these and are fitted to the times of all forms on 1410 products, dense and grouped, of all types and alignments, 1
+// to 16384 rows, 32 to 8192 channels and values, launched back to back and after other work: the form with the least such cost, which
+// is taken, ran 2.3 and 1.2 % longer than the best one there in the geometric mean.  Sums of 8-bit products are the same by
 // every form.
 enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, WIDE128, WIDE256, FORMS };
 struct FormCost {
-    int bm, bn, slots;  // tile, workgroups per round
+    int bm, bn, threads, slots;  // tile, workgroup, workgroups per round
     float start, fixed, cost, cost4, cost_odd, cost_f32, thin;  // costs: rows on 16 bytes, on 4, on less; f32 rows
 };
 constexpr FormCost FORM[FORMS] = {
-    {16, 16, 256, 5.8f, 1.1f, 3.0f, 1.9f, 3.8f, 3.0f, 0.66f},   {32, 16, 256, 6.0f, 0.9f, 3.9f, 4.6f, 4.3f, 5.5f, 1.f},     {32, 32, 256, 6.0f, 1.0f, 5.5f, 6.8f, 6.0f, 7.2f, 1.f},
-    {64, 64, 256, 6.7f, 1.9f, 9.2f, 16.f, 13.6f, 17.5f, 0.68f}, {128, 128, 256, 6.8f, 7.1f, 18.6f, 46.f, 40.f, 64.f, 0.59f}, {128, 128, 512, 8.9f, 8.3f, 28.f, 41.f, 41.f, 122.f, 0.77f},
-    {256, 256, 256, 10.2f, 15.f, 31.6f, 86.f, 84.f, 1e9f, 0.74f}};
+    {16, 16, 512, 256, 5.8f, 1.1f, 3.2f, 1.8f, 3.8f, 3.0f, 0.66f},   {32, 16, 512, 256, 6.1f, 0.9f, 4.1f, 4.1f, 4.3f, 5.4f, 0.98f},
+    {32, 32, 512, 256, 6.0f, 1.0f, 5.3f, 5.9f, 6.1f, 7.2f, 1.f},     {64, 64, 256, 256, 6.8f, 1.9f, 9.2f, 14.4f, 13.6f, 17.5f, 0.7f},
+    {128, 128, 512, 256, 5.9f, 7.1f, 18.9f, 42.f, 28.7f, 67.f, 0.72f}, {128, 128, 256, 512, 8.7f, 8.3f, 28.f, 41.f, 41.8f, 122.f, 0.75f},
+    {256, 256, 512, 256, 10.2f, 15.f, 31.8f, 0.f, 0.f, 0.f, 0.72f}};  // rows on 16 bytes only: in registers its loads do not fit
 
-// what the groups' rows can take in tiles of bm rows at most (every group but one may end inside a tile) ...
-long most_row_tiles(const LinearArgs &a, long bm) {
-    return a.offsets ? std::min<long>((a.m + bm - 1) / bm + a.groups - 1, a.m) : (a.m + bm - 1) / bm;
+// the workgroups of a launch: what the groups' rows can take in tiles at most (every group but one may end inside a tile) ...
+long workgroups(const LinearArgs &a, const FormCost &f) {
+    const long full = ((long)a.m + f.bm - 1) / f.bm, row_tiles = a.offsets ? std::min<long>(full + a.groups - 1, a.m) : full;
+    return (row_tiles * (((long)a.n + f.bn - 1) / f.bn) + 7) / 8 * 8;
 }
 
+// FORMS where no form's launch stays below 2^32 threads
 Form pick_form(const LinearArgs &a, bool f32, int align) {
     // ... and will take: the lengths are not known here.  So many groups have rows if the rows fall evenly; a group's last tile is half
     // full in the middle, and so is the last round
     const bool many = a.offsets && a.groups > 1;
     const float groups = many ? a.groups * (1.f - std::exp(-(float)a.m / a.groups)) : 1.f, rows = (float)a.m / groups;
     const float bytes = ((groups * a.n + a.m) * (float)a.kb + 2.f * a.m * a.n) / 5.1e6f;
-    int best = FEW11;
+    int best = FORMS;
     float least = 3.4e38f;
     for (int i = 0; i < FORMS; ++i) {
         const FormCost &f = FORM[i];
-        const float per_group = many ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)((a.m + f.bm - 1) / f.bm);
+        if (workgroups(a, f) > UINT32_MAX / f.threads || (i == WIDE256 && (f32 || align < 16))) continue;
+        const float per_group = many ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)(((long)a.m + f.bm - 1) / f.bm);
         const float all = groups * per_group * (float)((a.n + f.bn - 1) / f.bn) / (float)f.slots;
         const float rounds = many ? std::max(1.f, all + 0.5f) : std::ceil(all);
         const float thin = f.thin + (1.f - f.thin) * std::min(1.f, rows / (float)f.bm);
@@ -103,10 +109,9 @@ Form pick_form(const LinearArgs &a, bool f32, int align) {
 template <int T, int AL>
 int launch(LinearArgs a, hipStream_t s) {
     const Form f = pick_form(a, T == F32, AL);
-    const long row_tiles = most_row_tiles(a, FORM[f].bm), n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
-    PB_CHECK(row_tiles < (INT_MAX - 8) / n_tiles, PB_ERR_INVALID, "linear: %d x %d is more tiles than one launch takes", a.m, a.n);
-    a.n_tiles = (int)n_tiles;
-    const dim3 grid((unsigned)((row_tiles * n_tiles + 7) / 8 * 8));
+    PB_CHECK(f != FORMS, PB_ERR_INVALID, "linear: %d x %d is more than one launch takes", a.m, a.n);
+    a.n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
+    const dim3 grid((unsigned)workgroups(a, FORM[f]));
     constexpr bool DW = AL >= 4;
     switch (f) {
         case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, DW>), grid, dim3(512), 0, s, a); break;
@@ -116,7 +121,7 @@ int launch(LinearArgs a, hipStream_t s) {
         case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, AL == 16>), grid, dim3(512), 0, s, a); break;
         case WIDE128: hipLaunchKernelGGL((k_linear_wide<T, 128, 128, 64, 64, 2, 3, AL == 16>), grid, dim3(256), 0, s, a); break;
         default:
-            if constexpr (T != F32) hipLaunchKernelGGL((k_linear_wide<T, 256, 256, 128, 64, 2, AL == 16 ? 7 : 1, AL == 16>), grid, dim3(512), 0, s, a);
+            if constexpr (T != F32 && AL == 16) hipLaunchKernelGGL((k_linear_wide<T, 256, 256, 128, 64, 2, 7, true>), grid, dim3(512), 0, s, a);
             break;
     }
     PB_HIP(hipGetLastError());
@@ -140,12 +145,12 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     PB_CHECK(i8 || !bad_type(type), PB_ERR_INVALID, "%s: unknown type %d", who, type);
     PB_CHECK(!bad_type(y_type), PB_ERR_INVALID, "%s: unknown output type %d (f32, bf16, f16)", who, y_type);
     PB_CHECK(act >= PB_ACT_NONE && act <= PB_ACT_TANH, PB_ERR_INVALID, "%s: unknown activation %d", who, act);
-    PB_CHECK(m <= INT_MAX && x_total <= INT_MAX && y_total <= INT_MAX, PB_ERR_INVALID, "%s: more than 2^31 - 1 rows", who);
+    PB_CHECK(m <= MAX_ROWS && x_total <= MAX_ROWS && y_total <= MAX_ROWS, PB_ERR_INVALID, "%s: more than 2^31 - 257 rows", who);
     PB_CHECK(n <= (uint32_t)INT_MAX / 2 && k <= 1u << 28, PB_ERR_INVALID, "%s: n = %u, k = %u is out of range", who, n, k);
     PB_CHECK(!i8 || k <= PB_LINEAR_I8_MAX_K, PB_ERR_INVALID, "%s: k = %u would overflow 32-bit sums (at most %u)", who, k, PB_LINEAR_I8_MAX_K);
     PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
-    PB_CHECK(ldx >= k && ldw >= k && ldy >= n && ldx <= MAX_LD && ldw <= MAX_LD && ldy <= MAX_LD, PB_ERR_INVALID,
-             "%s: rows of %u inputs and %u outputs do not fit their strides", who, k, n);
+    PB_CHECK(ldx >= k && ldw >= k && ldy >= n && ldx <= MAX_LD && ldw <= MAX_LD && ldy <= MAX_LD && fits(x_total, ldx) && fits((uint64_t)groups * n, ldw) && fits(y_total, ldy), PB_ERR_INVALID,
+             "%s: rows of %u inputs and %u outputs do not fit their strides, or these the memory", who, k, n);
     if (m == 0 || n == 0) return PB_OK;
     const int size = type_bytes(type), y_size = type_bytes(y_type);
     PB_CHECK(y && (k == 0 || (x && w)), PB_ERR_INVALID, "%s: null buffer", who);
@@ -160,6 +165,10 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     const uint64_t y_bytes = extent(y_total, ldy, n, y_size);
     PB_CHECK(!overlap(y, y_bytes, x, extent(x_total, ldx, k, size)) && !overlap(y, y_bytes, w, extent((uint64_t)groups * n, ldw, k, size)), PB_ERR_INVALID,
              "%s: y overlaps an operand", who);
+    PB_CHECK(!(i8 && (overlap(y, y_bytes, x_scale, x_total * 4) || overlap(y, y_bytes, w_scale, (uint64_t)groups * n * 4))) &&
+                 !overlap(y, y_bytes, bias, (uint64_t)groups * n * 4) && !overlap(y, y_bytes, offsets, (groups + 1ull) * 4) &&
+                 !overlap(y, y_bytes, x_rows, m * 4) && !overlap(y, y_bytes, y_rows, m * 4),
+             PB_ERR_INVALID, "%s: y overlaps a scale, the bias or an index array", who);
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
     LinearArgs a;
@@ -193,15 +202,21 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     }
 }
 
-// a wave per row where the row fits its registers and there are rows for every CU, else a workgroup of four
+// a wave per row where the row fits its registers and there are rows for every CU, else a workgroup of four; launches of fewer than
+// 2^32 threads
 template <int T>
 void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale, hipStream_t s) {
-    const uint8_t *px = static_cast<const uint8_t *>(x);
-    int8_t *pc = static_cast<int8_t *>(codes);
     constexpr uint32_t V = T == F32 ? 4 : 8;
     const long lx = (long)ldx * type_bytes(T), lc = (long)ldc;
-    if (m >= 1024 && k <= 64 * V * 8) hipLaunchKernelGGL((k_quantize_rows<T, 64, 8>), dim3((unsigned)((m + 3) / 4)), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
-    else hipLaunchKernelGGL((k_quantize_rows<T, 256, 4>), dim3((unsigned)m), dim3(256), 0, s, px, (int)m, (int)k, lx, pc, lc, scale);
+    const bool waves = m >= 1024 && k <= 64 * V * 8;
+    const uint64_t most = waves ? 4ull << 23 : 1ull << 23;
+    for (uint64_t r = 0; r < m; r += most) {
+        const uint8_t *px = static_cast<const uint8_t *>(x) + r * lx;
+        int8_t *pc = static_cast<int8_t *>(codes) + r * lc;
+        const int rows = (int)std::min(most, m - r);
+        if (waves) hipLaunchKernelGGL((k_quantize_rows<T, 64, 8>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, px, rows, (int)k, lx, pc, lc, scale + r);
+        else hipLaunchKernelGGL((k_quantize_rows<T, 256, 4>), dim3((unsigned)rows), dim3(256), 0, s, px, rows, (int)k, lx, pc, lc, scale + r);
+    }
 }
 
 }  // namespace
@@ -211,8 +226,8 @@ extern "C" {
 int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64_t m, uint32_t k, uint64_t ldx, void *codes, uint64_t ldc, float *scale) {
     const char *who = "pb_quantize_rows";
     PB_CHECK(!bad_type(x_type), PB_ERR_INVALID, "%s: unknown type %d (f32, bf16, f16)", who, x_type);
-    PB_CHECK(m <= INT_MAX && k <= 1u << 28, PB_ERR_INVALID, "%s: m = %llu, k = %u is out of range", who, (unsigned long long)m, k);
-    PB_CHECK(ldx >= k && ldc >= k && ldx <= MAX_LD && ldc <= MAX_LD, PB_ERR_INVALID, "%s: rows of %u values do not fit their strides", who, k);
+    PB_CHECK(m <= MAX_ROWS && k <= 1u << 28, PB_ERR_INVALID, "%s: m = %llu, k = %u is out of range", who, (unsigned long long)m, k);
+    PB_CHECK(ldx >= k && ldc >= k && ldx <= MAX_LD && ldc <= MAX_LD && fits(m, ldx) && fits(m, ldc), PB_ERR_INVALID, "%s: rows of %u values do not fit their strides, or these the memory", who, k);
     if (m == 0) return PB_OK;
     const int size = type_bytes(x_type);
     PB_CHECK(scale && (k == 0 || (x && codes)), PB_ERR_INVALID, "%s: null buffer", who);
@@ -239,7 +254,7 @@ int pb_linear_i8(int device, void *stream, const void *x, uint64_t ldx, const fl
 
 int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32_t groups, int *offsets, int *order) {
     const char *who = "pb_group_rows";
-    PB_CHECK(m <= INT_MAX, PB_ERR_INVALID, "%s: more than 2^31 - 1 rows", who);
+    PB_CHECK(m <= MAX_ROWS, PB_ERR_INVALID, "%s: more than 2^31 - 257 rows", who);
     PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
     PB_CHECK(offsets && (m == 0 || (group && order)), PB_ERR_INVALID, "%s: null buffer", who);
     PB_CHECK(!misaligned(group, 4) && !misaligned(offsets, 4) && !misaligned(order, 4), PB_ERR_INVALID, "%s: a buffer is not aligned to 4 bytes", who);

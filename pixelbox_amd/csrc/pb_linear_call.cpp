@@ -46,6 +46,12 @@ void *stream_of(int device) { return c10::hip::getCurrentHIPStream((c10::DeviceI
 const float *floats(const Tensor *t) { return t ? static_cast<const float *>(t->data_ptr()) : nullptr; }
 const int *ints(const Tensor *t) { return t ? static_cast<const int *>(t->data_ptr()) : nullptr; }
 
+// an output as a kernel argument: its version is counted up, so that a backward pass that saved the old values says so
+void *written(const Tensor *t) {
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+    return t->data_ptr();
+}
+
 // the call's status as a number; None for a call that is not the usual one
 PyObject *status(int rc) { return PyLong_FromLong(rc); }
 #define PB_USUAL(cond) \
@@ -72,8 +78,8 @@ PyObject *quantize_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int dev = (int)x->get_device();
     const int64_t m = x->size(0), k = x->size(1);
     PB_USUAL(float_matrix(x, dev, m, k) && matrix(codes, at::kChar, dev, m, k) && vector(scale, at::kFloat, dev, m) && k < (1ll << 31));
-    return status(f_quantize(dev, stream_of(dev), x->data_ptr(), float_type(*x), (uint64_t)m, (uint32_t)k, (uint64_t)k, codes->data_ptr(), (uint64_t)k,
-                             static_cast<float *>(scale->data_ptr())));
+    return status(f_quantize(dev, stream_of(dev), x->data_ptr(), float_type(*x), (uint64_t)m, (uint32_t)k, (uint64_t)k, written(codes), (uint64_t)k,
+                             static_cast<float *>(written(scale))));
 }
 
 // (x, x_scale, w, w_scale, bias or None, act, out)
@@ -88,7 +94,7 @@ PyObject *linear_i8(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     const long act = PyLong_AsLong(a[5]);
     if (act == -1 && PyErr_Occurred()) return nullptr;
     return status(f_linear_i8(dev, stream_of(dev), x->data_ptr(), (uint64_t)k, floats(xs), w->data_ptr(), (uint64_t)k, floats(ws), floats(bias), (int)act,
-                              out->data_ptr(), float_type(*out), (uint64_t)n, (uint64_t)m, (uint32_t)n, (uint32_t)k));
+                              written(out), float_type(*out), (uint64_t)n, (uint64_t)m, (uint32_t)n, (uint32_t)k));
 }
 
 // (group, groups, offsets, order)
@@ -105,8 +111,8 @@ PyObject *group_rows(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int dev = (int)group->get_device();
     const int64_t m = group->size(0);
     PB_USUAL(vector(group, at::kInt, dev, m) && vector(offsets, at::kInt, dev, groups + 1) && vector(order, at::kInt, dev, m));
-    return status(f_group(dev, stream_of(dev), ints(group), (uint64_t)m, (uint32_t)groups, static_cast<int *>(offsets->data_ptr()),
-                          static_cast<int *>(order->data_ptr())));
+    return status(f_group(dev, stream_of(dev), ints(group), (uint64_t)m, (uint32_t)groups, static_cast<int *>(written(offsets)),
+                          static_cast<int *>(written(order))));
 }
 
 // (x, w, offsets, x_rows or None, y_rows or None, x_scale or None, w_scale or None, bias or None, act, out)
@@ -133,7 +139,7 @@ PyObject *linear_grouped(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     const long act = PyLong_AsLong(a[8]);
     if (act == -1 && PyErr_Occurred()) return nullptr;
     return status(f_grouped(dev, stream_of(dev), type, x->data_ptr(), (uint64_t)x_total, (uint64_t)k, floats(opt[2]), w->data_ptr(), (uint64_t)k, floats(opt[3]),
-                            floats(opt[4]), ints(offsets), (uint32_t)groups, ints(opt[0]), ints(opt[1]), (int)act, out->data_ptr(), float_type(*out),
+                            floats(opt[4]), ints(offsets), (uint32_t)groups, ints(opt[0]), ints(opt[1]), (int)act, written(out), float_type(*out),
                             (uint64_t)y_total, (uint64_t)n, (uint64_t)m, (uint32_t)n, (uint32_t)k));
 }
 

@@ -199,7 +199,7 @@ __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
     const int rest = (int)(id - (long)band * BAND * a.n_tiles), bh = min(BAND, tiles_g - band * BAND);
     t.nt = rest / bh;
     t.r0 = lo_g + (band * BAND + rest % bh) * BM;
-    t.r1 = min(t.r0 + BM, hi_g);
+    t.r1 = t.r0 < lo_g ? t.r0 : min(t.r0 + BM, hi_g);  // offsets that do not ascend may count more tiles than an int holds: none then
     return t;
 }
 

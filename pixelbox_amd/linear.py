@@ -10,8 +10,9 @@ strides and devices are checked here, the work is queued on the tensors' device 
     offsets, order = group_rows(head_of_image, heads)            # images of a batch -> rows in the order of their heads
     y = linear_grouped(features, weights, offsets, rows=order, bias=bias, act="tanh")   # weights [heads, n, k]
 
-Rows may have any stride >= their length (a slice of a wider tensor), the last axis is contiguous.  Products have no gradient: an
-operand that requires one is refused.
+Rows may have any stride >= their length (a slice of a wider tensor), the last axis is contiguous; an output overlaps no other
+tensor of its call.  Products have no gradient: an operand that requires one is refused, and an output that a backward pass has
+saved is counted as written.
 """
 from __future__ import annotations
 
@@ -94,6 +95,13 @@ def _no_grad(*tensors) -> None:
         raise ValueError("these products have no gradient: an operand requires one (detach it, or call under torch.no_grad())")
 
 
+def _written(*tensors) -> None:
+    """the caller's tensors that a call writes: a backward pass that saved their old values is to say so"""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _act(act: str) -> int:
     if act not in _ACTS:
         raise ValueError(f"act is {act!r}, not one of {', '.join(_ACTS)}")
@@ -124,7 +132,7 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scale: tor
         raise ValueError(f"x has the shape {tuple(x.shape)}, not (rows, values)")
     m, k = x.shape
     _check(x, "x", (m, k), _FLOATS, dev)
-    _no_grad(x)
+    _no_grad(x, scale)
     if codes is None:
         codes = torch.empty((m, k), dtype=torch.int8, device=x.device)
     else:
@@ -134,6 +142,7 @@ def quantize_rows(x: torch.Tensor, codes: torch.Tensor | None = None, scale: tor
     else:
         _check(scale, "scale", (m,), (torch.float32,), dev)
     ldx, ldc = _ld(x, "x"), _ld(codes, "codes")
+    _written(codes, scale)
     _call(capi.lib().pb_quantize_rows(dev, _stream(dev), x.data_ptr(), _TYPES[x.dtype], m, k, ldx, codes.data_ptr(), ldc, scale.data_ptr()))
     return codes, scale
 
@@ -169,6 +178,7 @@ def linear_i8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: 
     else:
         _check(out, "out", (m, n), _FLOATS, dev)
     ldx, ldw, ldy = _ld(x, "x"), _ld(w, "w"), _ld(out, "out")
+    _written(out)
     _call(capi.lib().pb_linear_i8(dev, _stream(dev), x.data_ptr(), ldx, x_scale.data_ptr(), w.data_ptr(), ldw, w_scale.data_ptr(), _ptr(bias), code,
                                   out.data_ptr(), _TYPES[out.dtype], ldy, m, n, k))
     return out
@@ -199,6 +209,7 @@ def group_rows(group: torch.Tensor, groups: int, offsets: torch.Tensor | None = 
         order = torch.empty((m,), dtype=torch.int32, device=group.device)
     else:
         _check(order, "order", (m,), (torch.int32,), dev)
+    _written(offsets, order)
     _call(capi.lib().pb_group_rows(dev, _stream(dev), group.data_ptr(), m, groups, offsets.data_ptr(), order.data_ptr()))
     return offsets, order
 
@@ -276,6 +287,7 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
     if m == 0 or n == 0 or (out.shape[0] == 0 and y_rows is not None) or x_total == 0:
         return out
     ldx, ldy = _ld(x, "x"), _ld(out, "out")
+    _written(out)
     _call(capi.lib().pb_linear_grouped(dev, _stream(dev), _TYPES[x.dtype], x.data_ptr(), x_total, ldx, _ptr(x_scale), w.data_ptr(), ldw,
                                        _ptr(w_scale), _ptr(bias), offsets.data_ptr(), groups, _ptr(x_rows), _ptr(y_rows), code, out.data_ptr(),
                                        _TYPES[out.dtype], out.shape[0], ldy, m, n, k))

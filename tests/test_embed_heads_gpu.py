@@ -152,6 +152,34 @@ def test_refusals(emb):
     emb.heads_device(**{**ok, "n": 0})
 
 
+def test_buffers_that_overlap_are_refused(emb):
+    img = images(0, 4)
+    w, head = torch.zeros((2, 8, 1280), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    buf = torch.zeros(64, device="cuda")
+    ok = dict(d_rgb_ptr=img.data_ptr(), n=4, w_type=0, d_w_ptr=w.data_ptr(), heads=2, d=8, d_head_ptr=head.data_ptr(), d_out_u8_ptr=buf.data_ptr() + 128,
+              d_out_f32_ptr=buf.data_ptr())
+    for change in (dict(d_out_u8_ptr=buf.data_ptr() + 127), dict(d_out_u8_ptr=head.data_ptr()), dict(d_out_f32_ptr=head.data_ptr(), d_out_u8_ptr=0),
+                   dict(d_out_f32_ptr=w.data_ptr() + 32), dict(d_bias_ptr=buf.data_ptr() + 64)):
+        with pytest.raises(capi.PixelboxError) as e:
+            emb.heads_device(**{**ok, **change})
+        assert e.value.code == -1, change
+    with pytest.raises(capi.PixelboxError):
+        emb.features_device(img.data_ptr(), 4, img.data_ptr() + 16)
+    emb.heads_device(**ok)
+
+
+def test_heads_of_growing_width(emb):
+    """bytes alone: the values go through a buffer of the embedder's that grows with the widest heads so far"""
+    g = torch.Generator().manual_seed(8)
+    img = images(120, 20)
+    head = (torch.arange(20) % 3).to(torch.int32).cuda()
+    for d in (16, 200, 24, 1000, 16):
+        w = (torch.randn((3, d, 1280), generator=g) * 0.05).cuda()
+        only, _ = run(emb, img, head, w, None, f32=False)
+        both, _ = run(emb, img, head, w, None)
+        assert torch.equal(only, both)
+
+
 def test_hashes_of_a_head_go_into_its_index(emb):
     """images -> heads -> the index of each collection -> a query answers as the oracle does on those hashes"""
     g = torch.Generator().manual_seed(3)

@@ -48,6 +48,11 @@ REFUSED = [
     (group, dict(order=P + 4)), (group, dict(offsets=R)), (group, dict(m=1 << 31)), (group, dict(group=P + 2)),
     (grouped, dict(type=4)), (grouped, dict(type=3)), (grouped, dict(yt=3)), (grouped, dict(groups=0)), (grouped, dict(groups=1025)), (grouped, dict(offsets=None)),
     (grouped, dict(offsets=Q + 1)), (grouped, dict(xr=None, xt=99)), (grouped, dict(yr=None, ytot=99)), (grouped, dict(xt=0)), (grouped, dict(ytot=0)),
+    (quantize, dict(m=(1 << 31) - 256)), (quantize, dict(m=1 << 30, ldx=1 << 40)), (i8, dict(m=(1 << 31) - 256)), (i8, dict(m=1 << 30, ldy=1 << 40)),
+    (group, dict(m=(1 << 31) - 256)), (grouped, dict(m=(1 << 31) - 256, xt=(1 << 31) - 257, ytot=(1 << 31) - 257)), (grouped, dict(ldw=1 << 40, n=1 << 20, ldy=1 << 20)),
+    (grouped, dict(xt=(1 << 31) - 256)), (grouped, dict(ytot=(1 << 31) - 256)),
+    (i8, dict(xs=S + 64)), (i8, dict(ws=S)), (i8, dict(bias=S + 4)), (grouped, dict(offsets=S + 8)), (grouped, dict(xr=S)), (grouped, dict(yr=S + 64)),
+    (grouped, dict(bias=S)),
     (grouped, dict(x=P + 1)), (grouped, dict(y=P + 64)), (grouped, dict(y=R)), (grouped, dict(ldx=63)), (grouped, dict(ldw=10)), (grouped, dict(ldy=1)),
 ]
 

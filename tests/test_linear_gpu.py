@@ -161,6 +161,28 @@ def test_every_form_at_every_remainder(kind, m, n):
         assert (y.double() - want).abs().amax().item() <= 2e-5 * scale
 
 
+# the forms that the sizes above leave out for some type or alignment
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n", [(24, 3000), (300, 2048), (1300, 1400), (1000, 4096), (2048, 2048), (1500, 3000), (3000, 3001)])
+def test_every_form_at_every_alignment(kind, m, n):
+    size = {"f32": 4, "bf16": 2, "f16": 2, "i8": 1}[kind]
+    k = 1040 // size
+    x, xs, w, ws, b = grouped_case(kind, m, 1, n, k, m + n)
+    want = x.double() @ w[0].double().t()
+    if kind == "i8":
+        want = want * xs.double()[:, None] * ws[0].double()
+    want += b[0].double()
+    # a sum of k products rounds at most k times, each time by 2^-24 of at most the sum of the products' magnitudes; scales, bias and the
+    # 64-bit result's own products: less than 8 more
+    most = (k + 8) * 2.0 ** -24 * (x.double().abs() @ w[0].double().abs().t() * (1 if xs is None else xs.double()[:, None] * ws[0].double()) + b[0].double().abs())
+    offsets = torch.tensor([0, m], dtype=torch.int32).cuda()
+    for ld, shift in ((k, 0), (k + 16 // size, 16 // size), (k + 4 // size, 0), (k, 4 // size), (k + 1, 0), (k + 8 // size, 1)):
+        y = torch.full((m, n), float("nan"), device="cuda")
+        wl = strided(w[0], ld, shift)
+        linear.linear_grouped(strided(x, ld, shift), wl.as_strided((1, n, k), (n * ld, ld, 1), wl.storage_offset()), offsets, x_scale=xs, w_scale=ws, bias=b, out=y)
+        assert ((y.double() - want).abs() <= most).all(), (ld, shift)
+
+
 def test_linear_i8_sums_are_exact_at_the_largest_k():
     k = capi.PB_LINEAR_I8_MAX_K
     x = torch.full((2, k), -128, dtype=torch.int8, device="cuda")
@@ -226,6 +248,27 @@ def test_linear_i8_rows_beyond_32_bits():
     check_codes(out, c, s)
 
 
+def test_more_rows_than_one_launch_has_threads_for():
+    """quantize_rows: in several launches; linear_i8: by larger tiles.  Few values and channels, rows by the hundred million"""
+    m, k = 40_000_000, 2
+    x = torch.empty((m, k), dtype=torch.float16, device="cuda")
+    r = torch.arange(m, device="cuda")
+    x[:, 0] = (r % 1009 + 1).to(torch.float16)
+    x[:, 1] = -(r % 127).to(torch.float16)
+    c, s = linear.quantize_rows(x)
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 1, m - 5, m - 1], device="cuda")
+    check_codes(x[at], c[at], s[at])
+    by = torch.full((1,), 127.0, device="cuda")  # a tensor: torch divides by a number by multiplying with its reciprocal
+    assert torch.equal(s, torch.clamp(torch.maximum(x[:, 0], -x[:, 1]).float() / by, min=2.0 ** -126))
+    del x, c, s, r
+    m = 140_000_000  # 16 rows a workgroup of 512 threads would be more than 2^32 threads
+    x = (torch.arange(m, device="cuda") % 251 - 125).to(torch.int8)[:, None]
+    one = torch.ones(m, device="cuda")
+    w, ws = torch.tensor([[3]], dtype=torch.int8, device="cuda"), torch.tensor([0.5], device="cuda")
+    y = linear.linear_i8(x, one, w, ws, dtype=torch.float16)
+    assert torch.equal(y, x.to(torch.float16) * 1.5)  # 375 / 2 at most: halves, exact in f16
+
+
 # ---- group_rows --------------------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("m,groups", [(0, 3), (1, 1), (1, 5), (63, 2), (64, 64), (257, 7), (4096, 1024), (5000, 33), (20001, 300)])
@@ -253,6 +296,19 @@ def test_group_rows_all_alike(value):
     offsets, order = linear.group_rows(g, 3)
     assert torch.equal(order.cpu(), torch.arange(777, dtype=torch.int32))
     assert offsets.cpu().tolist() == [0] + [777 if 0 <= value <= i else 0 for i in range(3)]
+
+
+@pytest.mark.parametrize("m", [100, 3001, 20000, 32769, 60000, 65537, 100001, 131072, 150000])
+@pytest.mark.parametrize("groups", [1, 2, 4, 6])
+def test_group_rows_of_dense_and_sparse_groups(m, groups):
+    """one group with most rows, in runs and single, beside small ones: both ways of writing a group's rows"""
+    g = torch.randint(0, 40, (m,), generator=gen(m + groups), dtype=torch.int32)
+    g = torch.where(g < groups, g, torch.zeros_like(g))
+    g[m // 3: m // 2] = groups - 1
+    g[m // 2: m // 2 + m // 7] = -1
+    offsets, order = linear.group_rows(g.cuda(), groups)
+    want_offsets, want_order = ref.group(g, groups)
+    assert torch.equal(offsets.cpu(), want_offsets) and torch.equal(order.cpu(), want_order)
 
 
 # ---- linear_grouped ----------------------------------------------------------------------------------------------------------------------
@@ -426,6 +482,16 @@ def test_captured_and_replayed(kind):
         assert torch.equal(out, want), i
 
 
+def test_offsets_that_do_not_ascend_stay_inside():
+    """groups that overlap, run backwards or end before they begin: some rows are written more than once or never, none outside"""
+    m, groups, n, k = 500, 8, 40, 64
+    x, xs, w, ws, b = grouped_case("bf16", m, groups, n, k, 5)
+    for bad in ([0, 500, 0, 500, 0, 500, 0, 500, 0], [500, 400, 300, 200, 100, 50, 20, 10, 0], [-(2**31), 2**31 - 1, 7, 9, 9, 2**31 - 1, -1, 3, 500]):
+        out = torch.full((m + 20, n), 5.0, device="cuda")
+        linear.linear_grouped(x, w, torch.tensor(bad, dtype=torch.int32, device="cuda"), bias=b, out=out[10:m + 10])
+        assert (out[:10] == 5).all() and (out[m + 10:] == 5).all() and torch.isfinite(out).all()
+
+
 def test_another_stream_and_two_threads():
     x, xs, w, ws, b = i8_case(600, 500, 700, 77)
     want = linear.linear_i8(x, xs, w, ws, bias=b, act="tanh")
@@ -465,6 +531,36 @@ def test_no_gradient_is_refused_not_lost():
         linear.quantize_rows(x)
     with torch.no_grad():
         assert linear.linear_grouped(x, w, offsets).shape == (4, 5)
+
+
+@pytest.mark.parametrize("short", [True, False])
+def test_a_backward_pass_sees_that_an_output_was_written(short, monkeypatch):
+    if not short:
+        monkeypatch.setattr(linear, "_compiled", False)
+    x, xs, w, ws, b = i8_case(6, 8, 32, 1)
+    a, out = torch.ones((6, 8), device="cuda", requires_grad=True), torch.ones((6, 8), device="cuda")
+    loss = (a * out).sum()  # saves out
+    linear.linear_i8(x, xs, w, ws, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before = [t._version for t in (out, xs)]
+    linear.linear_grouped(x, w[None], torch.tensor([0, 6], dtype=torch.int32, device="cuda"), x_scale=xs, w_scale=ws[None], out=out)
+    assert [t._version for t in (out, xs)] == [before[0] + 1, before[1]]
+    codes_, scale = linear.quantize_rows(out)
+    v = codes_._version, scale._version
+    linear.quantize_rows(out, codes=codes_, scale=scale)
+    offsets, order = linear.group_rows(torch.zeros(5, dtype=torch.int32, device="cuda"), 1)
+    u = offsets._version, order._version
+    linear.group_rows(torch.zeros(5, dtype=torch.int32, device="cuda"), 1, offsets=offsets, order=order)
+    assert (codes_._version, scale._version) == (v[0] + 1, v[1] + 1) and (offsets._version, order._version) == (u[0] + 1, u[1] + 1)
+    with torch.inference_mode():
+        inside = torch.empty((6, 8), device="cuda")
+        linear.linear_i8(x, xs, w, ws, out=inside)
+    linear.linear_i8(x, xs, w, ws, out=inside)  # has no version to count
+    assert torch.equal(inside, out)
+    grad = torch.ones(6, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        linear.quantize_rows(out, scale=grad)
 
 
 @pytest.mark.parametrize("kind", KINDS)
