@@ -860,9 +860,11 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
 // others: no scratch memory, no atomics, one launch, one possible result.  A first walk, four consecutive rows per lane, turns each
 // comparison into a lane mask: the counts come from the scalar unit's bit counts, the masks of matching rows go to LDS -- four
 // vector instructions for 64 rows, which is what bounds it (131072 rows, 256 groups: 27 us with a bit per lane put together by vector
-// instructions).  Then every thread takes a contiguous run of words of 32 rows, learns by a prefix sum over the bit counts where its
-// rows go, and writes them.  Its stores go to lines apart, so the waves of a group that has a fifth of the rows or more write 64 rows'
-// worth side by side instead (131072 rows of one group: 74 us by threads, 21 by waves; of 8 groups: 15.6 and 20.8).  Rows beyond one LDS map's 8192 per wave are walked a second time, map by map.
+// instructions).  Then every lane takes words of 32 rows, learns by prefix sums over the bit counts where its rows go, and lists
+// them in LDS, from where the wave writes whole lines: rows written straight from the lanes that found them go to lines apart (131072
+// rows of one group: 74 us).  Where half of a wave's 2048 rows and more are the group's, 64 rows' worth are written at once instead
+// (one group 21 us, 8 groups 13, 256 groups 15; 256 groups of uneven sizes and a tenth of the rows without one 17.8: the workgroup with
+// the most rows is the last).  Rows beyond one LDS map's 8192 per wave are walked a second time, map by map.
 // As unsigned numbers, rows of no group are >= groups: a row is before group g if it is < g.
 // v with the wave-uniform `value` in one lane: v_writelane_b32 as the compiler's intrinsic, which has no builtin of its own (as inline
 // asm the compiler leaves out the two wait states between the comparison that writes the scalar register and this read of it)
@@ -871,8 +873,9 @@ extern "C" __device__ __attribute__((const)) int pb_writelane(int value, int lan
 template <int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 8) void k_group_rows(const int32_t *__restrict__ group, int m, int groups, int vec, int32_t *__restrict__ offsets,
                                                               int32_t *__restrict__ order) {
-    constexpr int NTHR = 64 * WAVES, CHUNK = WAVES * 8192;
+    constexpr int NTHR = 64 * WAVES, CHUNK = WAVES * 8192, STAGE = 1024;
     __shared__ uint32_t s_mask[CHUNK / 32];  // per 256 rows eight words: rows 4 l + i of lane l at bit l of pair i
+    __shared__ uint16_t s_rows[WAVES][STAGE];
     __shared__ int s_lt[WAVES], s_eq[WAVES];
     const unsigned g = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -955,51 +958,50 @@ __global__ __launch_bounds__(64 * WAVES, 8) void k_group_rows(const int32_t *__r
                 }
                 return bits;
             };
+            const int w0 = wave * 64 * each;  // the wave's words: 64 at a time, one a lane
             uint32_t b[4];
-            int count = 0;
+            int inc[4], in_wave = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int w = tid * each + i;
+                const int w = w0 + i * 64 + lane;
                 b[i] = i < each && w < words ? word(w) : 0u;
-                count += __builtin_popcount(b[i]);
+                inc[i] = wave_prefix(__builtin_popcount(b[i]));
+                in_wave += __builtin_amdgcn_readlane(inc[i], 63);
             }
-            const int inc = wave_prefix(count);
-            if (lane == 63) s_eq[wave] = inc;
+            if (lane == 63) s_eq[wave] = in_wave;
             __syncthreads();
-            int before = 0, all = 0;
+            int to = first, all = 0;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                if (w < wave) before += s_eq[w];
+                if (w < wave) to += s_eq[w];
                 all += s_eq[w];
             }
-            if (5 * all < n) {  // every thread writes its own rows
-                int to = first + before + inc - count;
-                const int row0 = c * CHUNK + tid * each * 32;
+            first += all;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    for (uint32_t left = b[i]; left; left &= left - 1) order[to++] = row0 + i * 32 + __builtin_ctz(left);
-            } else {  // a wave goes through its threads' words 64 rows at a time and writes these side by side
-                int to = first + before, row = c * CHUNK + wave * 64 * each * 32;
-                auto put = [&](int low, int high) {
-                    const uint64_t mine = (uint64_t)(uint32_t)high << 32 | (uint32_t)low;
-                    const int at = to + __builtin_amdgcn_mbcnt_hi((uint32_t)high, __builtin_amdgcn_mbcnt_lo((uint32_t)low, 0u));
-                    if (__builtin_amdgcn_inverse_ballot_w64(mine)) order[at] = row + lane;
-                    to += __builtin_popcountll(mine);
-                    row += 64;
-                };
-                auto of_lane = [](uint32_t v, int l) { return __builtin_amdgcn_readlane((int)v, l); };
-                if (each == 1) {
+            for (int i = 0; i < 4; ++i) {
+                if (i >= each) break;
+                const int n_in = __builtin_amdgcn_readlane(inc[i], 63);
+                int row = c * CHUNK + (w0 + i * 64) * 32;
+                if (n_in <= STAGE) {  // every lane lists its own rows, and the wave writes them
+                    int at = inc[i] - __builtin_popcount(b[i]);
+                    for (uint32_t left = b[i]; left; left &= left - 1) s_rows[wave][at++] = (uint16_t)(lane * 32 + __builtin_ctz(left));
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // LDS keeps a wave's order
+                    for (int j = lane; j < n_in; j += 64) order[to + j] = row + s_rows[wave][j];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    to += n_in;
+                } else {  // 64 rows at a time, a lane each
+                    row += lane;
 #pragma unroll 4
-                    for (int l = 0; l < 64; l += 2) put(of_lane(b[0], l), of_lane(b[0], l + 1));
-                } else {
-#pragma unroll 4
-                    for (int l = 0; l < 64; ++l) {
-                        put(of_lane(b[0], l), of_lane(b[1], l));
-                        if (each == 4) put(of_lane(b[2], l), of_lane(b[3], l));
+                    for (int l = 0; l < 64; l += 2) {
+                        const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)b[i], l), high = (uint32_t)__builtin_amdgcn_readlane((int)b[i], l + 1);
+                        const uint64_t in = (uint64_t)high << 32 | low;
+                        const int at = to + __builtin_amdgcn_mbcnt_hi(high, __builtin_amdgcn_mbcnt_lo(low, 0u));
+                        if (__builtin_amdgcn_inverse_ballot_w64(in)) order[at] = row;
+                        to += __builtin_popcountll(in);
+                        row += 64;
                     }
                 }
             }
-            first += all;
         }
     };
     if (g == (unsigned)groups) run(std::true_type{});
