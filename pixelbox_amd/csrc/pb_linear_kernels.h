@@ -66,8 +66,7 @@ __device__ __forceinline__ void mma32(typename Acc<T>::q16 &c, const u32x4 &a, c
 
 // ---- loads and stores of any alignment ---------------------------------------------------------------------------------------------------
 // global_load / store_dwordx4 take any address; what that costs depends on the bound.  Tiles load a byte once for many products: on
-// 4 bytes or less they lose up to the difference between DMA and registers (4096^3 i8 by 256 x 256: 62 us aligned, 88 on 4 bytes, 98
-// odd).  The few forms live on loads, which go at full rate on 4 bytes and at a third off them (41 x 217 x 3903 f16: 26.6 us, with
+// 4 bytes or less they lose what the way through registers costs (4096^3 i8 by 128 x 128: 83 us aligned, 94 on 4 bytes, 125 odd).  The few forms live on loads, which go at full rate on 4 bytes and at a third off them (41 x 217 x 3903 f16: 26.6 us, with
 // 3904 values 10.1): there (DW false) the aligned words around the 16 bytes are read -- only such as hold at least one of them -- and
 // shifted into place (13.0 us; in tiles that costs more than it saves: 777 x 1003 x 1289 i8 12.6 us, plain 11.2).
 template <bool DW>
@@ -441,7 +440,7 @@ struct Loader {
 // ---- k_linear_tile: small tiles -- 64 x 64 or 128 x 128, waves of 32 x 32 or 64 x 32 ---------------------------------------------------------
 // For products with few tiles, where a step is short: a wave has one or two 32 x 32 matrix instructions to a 32-byte piece, and would
 // wait out an LDS read for each piece, so it reads a step's four pieces at once behind the step's one barrier; four LDS stages give
-// the loads three steps to arrive.  (4 pieces one after the other: 64 x 4096 x 4096 13.3 us instead of 12.8; two stages: weights out of
+// the loads three steps to arrive.  777 x 1003 x 1289 i8 13.6 us, 1024 x 1024 x 1008 7.6.  (4 pieces one after the other: 64 x 4096 x 4096 13.3 us instead of 12.8; two stages: weights out of
 // HBM, 128 x 8192 x 8192, 33.7 us instead of 22.0.)
 template <int T, int BM, int BN, int WM, int WN, int NST, bool DMA>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(const LinearArgs a) {
@@ -647,7 +646,10 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_wide(cons
 
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
 // For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
-// waves' partial sums meet in LDS and are added in wave order.
+// waves' partial sums meet in LDS and are added in wave order.  Bound by the weights out of HBM: 32 rows over 64 groups, 2048 x 2048 bf16
+// (210 MB of 25 groups in use) 42.6 us, 4.9 TB/s of the 5.1 that a large copy reaches; with weights in the caches by the way from a load
+// to the last sum (16 x 4096 x 4096 i8 7.2 us, 1 x 256 x 1280 4.3 of which 3.3 are any launch's).  Loads a turn ahead would cost
+// registers and with them waves: 40 us instead of 32 (evenly filled groups).
 template <int T, int MT, int NT, int NW, int U, bool DW>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     typedef typename Acc<T>::e E;
@@ -734,7 +736,8 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 // scale = max(max |x| / 127, 2^-126); code = x / scale to the nearest whole number, halves to the even one.  Without a division per
 // value, and exactly: x * (1 / scale) + 1.5 * 2^23, one fused multiply-add, is the whole number in the low bits (1 / scale is off by
 // half a unit in the last place, the quotient by less than 7.7e-6).  Only where it lies within 1e-5 of a half -- one value in 50 000 -- the
-// remainder x - r * scale decides, which a fused multiply-add gives exactly near scale / 2.  A row with an infinity or a NaN gets
+// remainder x - r * scale decides, which a fused multiply-add gives exactly near scale / 2.  Bound by HBM: 8192 x 1280 f32 (52 MB) 10.0
+// us, the rate of a large copy; 8192 x 8192 bf16 41.5.  A row with an infinity or a NaN gets
 // scale = NaN and codes 0, so that what is computed from it shows.
 constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
 __device__ __forceinline__ uint32_t code_exact(float x, float inv, float scale, float half) {
