@@ -647,7 +647,7 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_wide(cons
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
 // For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
 // waves' partial sums meet in LDS and are added in wave order.  Bound by the weights out of HBM: 32 rows over 64 groups, 2048 x 2048 bf16
-// (210 MB of 25 groups in use) 42.6 us, 4.9 TB/s of the 5.1 that a large copy reaches; with weights in the caches by the way from a load
+// (210 MB of 25 groups in use) 41 us, the 5.1 TB/s of a large copy; with weights in the caches by the way from a load
 // to the last sum (16 x 4096 x 4096 i8 7.2 us, 1 x 256 x 1280 4.3 of which 3.3 are any launch's).  Loads a turn ahead would cost
 // registers and with them waves: 40 us instead of 32 (evenly filled groups).
 template <int T, int MT, int NT, int NW, int U, bool DW>
@@ -657,6 +657,8 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     constexpr int BM = 16 * MT, BN = 16 * NT;
     constexpr int PITCH = BN + 4;
     __shared__ __attribute__((aligned(16))) E s_sum[NW][BM * PITCH];
+    __shared__ float s_xscale[BM], s_wscale[BN], s_bias[BN];
+    __shared__ int s_xrow[BM], s_yrow[BM];
     const Tile t = find_tile<BM, 1>(a);
     if (t.r0 >= t.r1) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -667,6 +669,22 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     for (int i = 0; i < MT; ++i) px[i] = a.x + (long)max(x_row_of(a, min(t.r0 + i * 16 + li, t.r1 - 1)), 0) * a.ldx + kq;
 #pragma unroll
     for (int j = 0; j < NT; ++j) pw[j] = a.w + ((long)t.g * a.n + min(c_base + j * 16 + li, a.n - 1)) * a.ldw + kq;
+    // what the end needs is on its way to LDS ahead of the operands: behind the sums it would cost two more trips to memory (512 rows
+    // over 8 groups, 256 x 1280 f32: 18.3 us instead of 17.4 with its group_rows)
+    auto to_lds = [](const float *from, float *to) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from, (__attribute__((address_space(3))) void *)to, 4, 0, 0);
+    };
+    if (wave == NW - 1 && lane < BM) {
+        const bool in = t.r0 + lane < t.r1;
+        const int xr = in ? x_row_of(a, t.r0 + lane) : -1, yr = in ? y_row_of(a, t.r0 + lane) : -1;
+        s_xrow[lane] = xr;
+        s_yrow[lane] = yr;
+        if constexpr (T == I8) to_lds(a.x_scale + max(xr, 0), s_xscale);
+    } else if (wave == NW - 2 && lane < BN) {
+        const long c = (long)t.g * a.n + min(c_base + lane, a.n - 1);
+        if constexpr (T == I8) to_lds(a.w_scale + c, s_wscale);
+        if (a.bias) to_lds(a.bias + c, s_bias);
+    }
     Q acc[NT][MT] = {};
     const int kb1 = a.kb;
     for (int kb = wave * 64 * U; kb < kb1; kb += 64 * U * NW) {
@@ -712,10 +730,12 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i) *reinterpret_cast<Q *>(&s_sum[wave][(i * 16 + li) * PITCH + j * 16 + (lane >> 4) * 4]) = acc[j][i];
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the loads into LDS
     __syncthreads();
     for (int q = tid; q < BM * BN / 4; q += 64 * NW) {
         const int r = q / (BN / 4), c = (q % (BN / 4)) * 4;
-        if (t.r0 + r >= t.r1) continue;
+        const int yr = s_yrow[r];
+        if (s_xrow[r] < 0 || yr < 0) continue;
         Q s = *reinterpret_cast<const Q *>(&s_sum[0][r * PITCH + c]);
 #pragma unroll
         for (int w = 1; w < NW; ++w) {
@@ -723,12 +743,14 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] += o[i];
         }
-        const int xr = x_row_of(a, t.r0 + r), yr = y_row_of(a, t.r0 + r);
-        if (xr < 0 || yr < 0) continue;
         Chan<T, 4> ch;
-        ch.load(a, t.g, c_base + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            ch.scale[i] = T == I8 ? s_wscale[c + i] : 1.0f;
+            ch.bias[i] = a.bias ? s_bias[c + i] : 0.0f;
+        }
         const E e[4] = {s[0], s[1], s[2], s[3]};
-        ch.finish(a, e, T == I8 ? a.x_scale[xr] : 1.0f, yr, c_base + c);
+        ch.finish(a, e, T == I8 ? s_xscale[r] : 1.0f, yr, c_base + c);
     }
 }
 
