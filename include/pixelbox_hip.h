@@ -455,7 +455,7 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
  * order of x; with only x_rows the groups' results lie packed, as the input of a next layer that has only y_rows.  offsets
  * (int[groups + 1]) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,
  * a row number outside x ([0, x_total)) or y ([0, y_total)) is skipped.  A row of x may be listed any number of times, a row of y
- * once (twice: either result stands).  Rows of y that are not listed are left as they are. */
+ * once (twice: either result stands, channel by channel).  Rows of y that are not listed are left as they are. */
 int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
                       const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
                       void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k);

@@ -221,8 +221,8 @@ def linear_grouped(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, rows
 
     x [rows of x, k] (f32, bf16, f16; int8 with x_scale [rows of x] and w_scale [groups, n]), w [groups, n, k], bias f32 [groups, n], offsets int32
     [groups + 1].  x_rows and y_rows (int32 [m], `rows` for both) name the row of x that is read and the row of out that is written at each place r;
-    without them it is r itself.  Rows of out that no place names are left as they are: zero where out is made here (m rows, or as many as x has
-    where y_rows is given)."""
+    without them it is r itself.  Rows of out that no place names are left as they are: zero where out is made here (m rows, or as many as x
+    has if that is more and y_rows is given)."""
     code = _act(act)
     if rows is not None:
         if x_rows is not None or y_rows is not None:

@@ -8,7 +8,7 @@ u = 2^-24 is the unit roundoff of f32.  The bounds count roundings:
   * + bias: u |v|;  both are multiplied by the activation's largest slope (SiLU 1.1, tanh 1);
   * the activation itself: SiLU = v * rcp(1 + exp2(-v log2 e)): the exponent's rounded product is off by |v| log2(e) u and a relative
     (|v| + 1) u of e^-v after that, exp2 and rcp are off by 2 u each, 1 + e^-v, the last product and log2(e)'s own rounding by u
-    each: (3 |v| + 8) u |silu(v)| in all; tanh = (1 - e) rcp(1 + e) with e = exp2(-2 |v| log2 e) off by (2 |v| + 2) u of itself, from
+    each: (3 |v| + 8) u |silu(v)| in all (below v = -87.3 the reciprocal may be 0: |v| 2^-126 more); tanh = (1 - e) rcp(1 + e) with e = exp2(-2 |v| log2 e) off by (2 |v| + 2) u of itself, from
     |v| = 0.4 on: the numerator is off by e / (1 - e) (2 |v| + 2) u <= 2.3 u there and rounds by u, the denominator by e / (1 + e) of
     the same <= 0.9 u and rounds by u, rcp 2 u, the product u: 8.2 u; below, the series to v^11: its next term 1 u, the last fused
     step 1 u, what comes before it (a sum below v^3 / 3, 6 % of the result) rounds by less than 1 u in all.  9 u |tanh v| covers both;

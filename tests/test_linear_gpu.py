@@ -172,9 +172,9 @@ def test_every_form_at_every_alignment(kind, m, n):
     if kind == "i8":
         want = want * xs.double()[:, None] * ws[0].double()
     want += b[0].double()
-    # a sum of k products rounds at most k times, each time by 2^-24 of at most the sum of the products' magnitudes; scales, bias and the
-    # 64-bit result's own products: less than 8 more
-    most = (k + 8) * 2.0 ** -24 * (x.double().abs() @ w[0].double().abs().t() * (1 if xs is None else xs.double()[:, None] * ws[0].double()) + b[0].double().abs())
+    # a sum of k products rounds at most k times, each time by a unit (2 x 2^-24) of at most the sum of the products' magnitudes; scales,
+    # bias and the 64-bit result's own products: less than 8 x 2^-24 more
+    most = (2 * k + 8) * 2.0 ** -24 * (x.double().abs() @ w[0].double().abs().t() * (1 if xs is None else xs.double()[:, None] * ws[0].double()) + b[0].double().abs())
     offsets = torch.tensor([0, m], dtype=torch.int32).cuda()
     for ld, shift in ((k, 0), (k + 16 // size, 16 // size), (k + 4 // size, 0), (k, 4 // size), (k + 1, 0), (k + 8 // size, 1)):
         y = torch.full((m, n), float("nan"), device="cuda")
@@ -393,6 +393,26 @@ def test_bad_device_data_touches_nothing_else(kind):
     twice = [int(rows[r]) for r in range(30, 60) if 0 <= int(rows[r]) < m]
     ok[twice] = True
     assert ok.all()
+
+
+@pytest.mark.parametrize("name", ["tanh", "silu"])
+def test_activations_over_their_range(name):
+    """one value, one channel of weight 1: the activation of exactly that value; around 0.4, where tanh changes its formula, closely"""
+    v = torch.cat([torch.logspace(-30, 2, 150_000, dtype=torch.float64), torch.linspace(0.3999, 0.4001, 20_000, dtype=torch.float64),
+                   torch.linspace(0.01, 12.0, 100_000, dtype=torch.float64)]).float()
+    v = torch.cat([v, -v])
+    y = linear.linear_grouped(v[:, None].cuda(), torch.ones((1, 1, 1), device="cuda"), torch.tensor([0, v.numel()], dtype=torch.int32, device="cuda"), act=name)
+    x = v.double()
+    want = ref.act(x, name)
+    factor = 9 if name == "tanh" else 3 * x.abs() + 8  # the bounds of linear_ref, and half a unit for a result that no f32 is
+    # results below the smallest normal value may be zero; SiLU = v / (1 + e^-v): the reciprocal may be, below 2^-126 (v < -87.3), and
+    # times |v| that is all of the result
+    below = 2.0 ** -126 * (1 if name == "tanh" else torch.clamp(x.abs(), min=1.0))
+    assert ((y[:, 0].cpu().double() - want).abs() <= (factor + 1) * 2.0 ** -24 * want.abs() + below).all()
+    ends = torch.tensor([0.0, -0.0, float("inf"), 3e38, -3e38, float("nan")])
+    y = linear.linear_grouped(ends[:, None].cuda(), torch.ones((1, 1, 1), device="cuda"), torch.tensor([0, 6], dtype=torch.int32, device="cuda"), act=name)[:, 0].cpu()
+    assert y[0] == 0 and y[1] == 0 and torch.isnan(y[5])
+    assert y[2:5].tolist() == ([1.0, 1.0, -1.0] if name == "tanh" else [float("inf"), ends[3].item(), 0.0])
 
 
 def test_rows_of_x_may_be_listed_often():
