@@ -285,7 +285,8 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
  * quantiser of efficientnet.rs:39, all on the embedder's stream (contract as pb_embed_batch_device).  All pointers are DEVICE memory.
  * type: PB_TYPE_F32 (d_w: f32[heads][d][1280]) or PB_TYPE_I8 (int8, with d_w_scale f32[heads][d]: pb_quantize_rows over the weights'
  * rows); d_bias: f32[heads][d] or NULL; d_head: int[n].  d_out_u8: uint8[n][d], d_out_f32: f32[n][d], either may be NULL.  Images
- * whose head is outside [0, heads) are left as they are in both; the outputs overlap neither each other nor d_head.  The f32 product is summed in plain f32 (the embedder's own Linear
+ * whose head is outside [0, heads) are left as they are in both; the outputs overlap neither each other nor d_head.  An image's hash does
+ * not depend on its batch, nor on the other heads.  The f32 product is summed in plain f32 (the embedder's own Linear
  * sums bf16 pieces): with the blob's own weights as the only head the values agree with pb_embed_batch to the embedding's tolerance,
  * not bit for bit.  An i8 head is off by the codes' rounding: half a code of 254 per feature and weight. */
 int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
@@ -450,7 +451,8 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
 
 /* For every group g and position r in [offsets[g], offsets[g + 1]), with xr = x_rows ? x_rows[r] : r and yr likewise:
  *   y[yr] = act( (x[xr] . w[g]^T) (* x_scale[xr] * w_scale[g]) + bias[g] )
- * type: f32, bf16, f16 (products summed in f32) or i8 (as pb_linear_i8; x_scale f32[x_total] and w_scale f32[groups][n], ignored
+ * type: f32, bf16, f16 (products summed in f32, in an order that goes with the kernel chosen, which goes with the sizes: the last bits of
+ * a row may differ from one batch to another) or i8 (as pb_linear_i8; x_scale f32[x_total] and w_scale f32[groups][n], ignored
  * for the others).  w: [groups][n][ldw], bias: f32[groups][n] or NULL.  With x_rows = y_rows = pb_group_rows' order, y is in the
  * order of x; with only x_rows the groups' results lie packed, as the input of a next layer that has only y_rows.  offsets
  * (int[groups + 1]) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,

@@ -1,4 +1,4 @@
-// pb_common.h -- error plumbing shared by the HIP translation units (gfx950 only).
+// pb_common.h -- error plumbing shared by the HIP translation units (gfx950 only), and a call between two of them.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -48,5 +48,10 @@ struct DeviceGuard {
         if (prev >= 0) (void)hipSetDevice(prev);
     }
 };
+
+// pb_linear_grouped as the hash heads need it (pb_linear.hip): dense f32 or i8 operands, f32 results, tanh, rows read and written by
+// `order`.  An f32 sum is added in one order that depends on k alone, so that an image's hash does not depend on its batch.
+int linear_heads(int device, void *stream, int type, const void *x, const float *x_scale, const void *w, const float *w_scale, const float *bias,
+                 const int *offsets, uint32_t heads, const int *order, float *y, uint32_t n, uint32_t d, uint32_t k);
 
 }  // namespace pb

@@ -2014,9 +2014,7 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
         if ((rc = pb_quantize_rows(e->device, e->stream, e->hd_feat, PB_TYPE_F32, n, 1280, 1280, e->hd_codes, 1280, e->hd_scale))) return rc;
         x = e->hd_codes;
     }
-    if ((rc = pb_linear_grouped(e->device, e->stream, type, x, n, 1280, e->hd_scale, d_w, 1280, d_w_scale, d_bias, e->hd_offsets, heads, e->hd_order,
-                                e->hd_order, PB_ACT_TANH, val, PB_TYPE_F32, n, d, n, d, 1280)))
-        return rc;
+    if ((rc = pb::linear_heads(e->device, e->stream, type, x, e->hd_scale, d_w, d_w_scale, d_bias, e->hd_offsets, heads, e->hd_order, val, n, d, 1280))) return rc;
     if (d_out_u8) {
         hipLaunchKernelGGL(k_hash_rows, dim3((d + 255) / 256, n), dim3(256), 0, e->stream, val, d_head, (int)heads, (int)d, d_out_u8);
         PB_HIP(hipGetLastError());

@@ -74,13 +74,14 @@ constexpr FormCost FORM[FORMS] = {
     {256, 256, 512, 256, 10.2f, 15.f, 31.8f, 0.f, 0.f, 0.f, 0.72f}};  // rows on 16 bytes only: in registers its loads do not fit
 
 // the workgroups of a launch: what the groups' rows can take in tiles at most (every group but one may end inside a tile) ...
-long workgroups(const LinearArgs &a, const FormCost &f) {
-    const long full = ((long)a.m + f.bm - 1) / f.bm, row_tiles = a.offsets ? std::min<long>(full + a.groups - 1, a.m) : full;
-    return (row_tiles * (((long)a.n + f.bn - 1) / f.bn) + 7) / 8 * 8;
+long row_tiles(const LinearArgs &a, const FormCost &f) {
+    const long full = ((long)a.m + f.bm - 1) / f.bm;
+    return a.offsets ? std::min<long>(full + a.groups - 1, a.m) : full;
 }
+long workgroups(const LinearArgs &a, const FormCost &f) { return (row_tiles(a, f) * (((long)a.n + f.bn - 1) / f.bn) + 7) / 8 * 8; }
 
-// FORMS where no form's launch stays below 2^32 threads
-Form pick_form(const LinearArgs &a, bool f32, int align) {
+// FORMS where no form's launch stays below 2^32 threads; last: the largest form to choose from
+Form pick_form(const LinearArgs &a, bool f32, int align, Form last = WIDE256) {
     // ... and will take: the lengths are not known here.  So many groups have rows if the rows fall evenly; a group's last tile is half
     // full in the middle, and so is the last round
     const bool many = a.offsets && a.groups > 1;
@@ -88,7 +89,7 @@ Form pick_form(const LinearArgs &a, bool f32, int align) {
     const float bytes = ((groups * a.n + a.m) * (float)a.kb + 2.f * a.m * a.n) / 5.1e6f;
     int best = FORMS;
     float least = 3.4e38f;
-    for (int i = 0; i < FORMS; ++i) {
+    for (int i = 0; i <= last; ++i) {
         const FormCost &f = FORM[i];
         if (workgroups(a, f) > UINT32_MAX / f.threads || (i == WIDE256 && (f32 || align < 16))) continue;
         const float per_group = many ? std::max(1.f, rows / (float)f.bm + 0.5f) : (float)(((long)a.m + f.bm - 1) / f.bm);
@@ -107,15 +108,14 @@ Form pick_form(const LinearArgs &a, bool f32, int align) {
 
 // AL: every row of x and w starts on so many bytes (16: loads straight into LDS; 4; less)
 template <int T, int AL>
-int launch(LinearArgs a, hipStream_t s) {
-    const Form f = pick_form(a, T == F32, AL);
-    PB_CHECK(f != FORMS, PB_ERR_INVALID, "linear: %d x %d is more than one launch takes", a.m, a.n);
-    a.n_tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn;
-    const dim3 grid((unsigned)workgroups(a, FORM[f]));
+int launch_form(const LinearArgs &a, Form f, dim3 grid, hipStream_t s) {
     constexpr bool DW = AL >= 4;
+    // pieces of 64 bytes per wave and turn.  f32: the same in all three few forms, so that they add in one order (up to 1024 rows over 8
+    // groups, 256 x 1280: 16 x 16 and 32 x 16 outputs 2 % faster to 1 % slower than with 4, 32 x 32 with 4 pieces 3 to 8 % slower)
+    constexpr int U = T == F32 ? 2 : 4;
     switch (f) {
-        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, 4, DW>), grid, dim3(512), 0, s, a); break;
-        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, 4, DW>), grid, dim3(512), 0, s, a); break;
+        case FEW11: hipLaunchKernelGGL((k_linear_few<T, 1, 1, 8, U, DW>), grid, dim3(512), 0, s, a); break;
+        case FEW21: hipLaunchKernelGGL((k_linear_few<T, 2, 1, 8, U, DW>), grid, dim3(512), 0, s, a); break;
         case FEW22: hipLaunchKernelGGL((k_linear_few<T, 2, 2, 8, 2, DW>), grid, dim3(512), 0, s, a); break;
         case TILE64: hipLaunchKernelGGL((k_linear_tile<T, 64, 64, 32, 32, AL == 16 ? 4 : 2, AL == 16>), grid, dim3(256), 0, s, a); break;
         case TILE128: hipLaunchKernelGGL((k_linear_tile<T, 128, 128, 64, 32, 4, AL == 16>), grid, dim3(512), 0, s, a); break;
@@ -127,20 +127,35 @@ int launch(LinearArgs a, hipStream_t s) {
     PB_HIP(hipGetLastError());
     return PB_OK;
 }
-template <int T>
-int launch(const LinearArgs &a, hipStream_t s) {
-    const uint64_t low = (uint64_t)(uintptr_t)a.x | (uint64_t)(uintptr_t)a.w | (uint64_t)a.ldx | (uint64_t)a.ldw;
-    if (low % 16 == 0) return launch<T, 16>(a, s);
-    if constexpr (T != F32) {
-        if (low % 4 != 0) return launch<T, 1>(a, s);
+// one_order (f32): every sum is added in an order that depends on k alone -- by the few forms, in as many launches as the channels need
+template <int T, int AL>
+int launch(LinearArgs a, bool one_order, hipStream_t s) {
+    Form f = pick_form(a, T == F32, AL, one_order ? FEW22 : WIDE256);
+    if (one_order && f == FORMS) f = FEW22;
+    PB_CHECK(f != FORMS, PB_ERR_INVALID, "linear: %d x %d is more than one launch takes", a.m, a.n);
+    const long rows = row_tiles(a, FORM[f]), most = (UINT32_MAX / FORM[f].threads - 8) / rows;
+    const int tiles = (a.n + FORM[f].bn - 1) / FORM[f].bn, each = one_order ? (int)std::min<long>(tiles, std::max(1l, most)) : tiles;
+    for (a.nt0 = 0; a.nt0 < tiles; a.nt0 += each) {
+        a.n_tiles = std::min(each, tiles - a.nt0);
+        const int rc = launch_form<T, AL>(a, f, dim3((unsigned)((rows * a.n_tiles + 7) / 8 * 8)), s);
+        if (rc) return rc;
     }
-    return launch<T, 4>(a, s);
+    return PB_OK;
+}
+template <int T>
+int launch(const LinearArgs &a, bool one_order, hipStream_t s) {
+    const uint64_t low = (uint64_t)(uintptr_t)a.x | (uint64_t)(uintptr_t)a.w | (uint64_t)a.ldx | (uint64_t)a.ldw;
+    if (low % 16 == 0) return launch<T, 16>(a, one_order, s);
+    if constexpr (T != F32) {
+        if (low % 4 != 0) return launch<T, 1>(a, one_order, s);
+    }
+    return launch<T, 4>(a, one_order, s);
 }
 
 // what pb_linear_i8 and pb_linear_grouped have in common
 int linear(const char *who, int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w,
            uint64_t ldw, const float *w_scale, const float *bias, const int32_t *offsets, uint32_t groups, const int32_t *x_rows,
-           const int32_t *y_rows, int act, void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k) {
+           const int32_t *y_rows, int act, void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k, bool one_order = false) {
     const bool i8 = type == PB_TYPE_I8;
     PB_CHECK(i8 || !bad_type(type), PB_ERR_INVALID, "%s: unknown type %d", who, type);
     PB_CHECK(!bad_type(y_type), PB_ERR_INVALID, "%s: unknown output type %d (f32, bf16, f16)", who, y_type);
@@ -188,17 +203,17 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     a.m = (int)m;
     a.n = (int)n;
     a.groups = (int)groups;
-    a.n_tiles = 0;
+    a.n_tiles = a.nt0 = 0;
     a.x_total = (int)x_total;
     a.y_total = (int)y_total;
     a.act = act;
     a.y_type = y_type;
     hipStream_t s = static_cast<hipStream_t>(stream);
     switch (type) {
-        case PB_TYPE_F32: return launch<F32>(a, s);
-        case PB_TYPE_BF16: return launch<BF16>(a, s);
-        case PB_TYPE_F16: return launch<F16>(a, s);
-        default: return launch<I8>(a, s);
+        case PB_TYPE_F32: return launch<F32>(a, one_order, s);
+        case PB_TYPE_BF16: return launch<BF16>(a, false, s);
+        case PB_TYPE_F16: return launch<F16>(a, false, s);
+        default: return launch<I8>(a, false, s);
     }
 }
 
@@ -220,6 +235,12 @@ void launch_quantize(const void *x, uint64_t m, uint32_t k, uint64_t ldx, void *
 }
 
 }  // namespace
+
+int pb::linear_heads(int device, void *stream, int type, const void *x, const float *x_scale, const void *w, const float *w_scale, const float *bias,
+                     const int *offsets, uint32_t heads, const int *order, float *y, uint32_t n, uint32_t d, uint32_t k) {
+    return linear("pb_embed_heads_device", device, stream, type, x, n, k, x_scale, w, k, w_scale, bias, offsets, heads, order, order, PB_ACT_TANH, y,
+                  PB_TYPE_F32, n, d, n, d, k, true);
+}
 
 extern "C" {
 

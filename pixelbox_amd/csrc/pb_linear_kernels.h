@@ -115,7 +115,8 @@ struct LinearArgs {
     uint8_t *y;
     long ldx, ldw, ldy;      // bytes between rows
     int kb;                  // bytes summed over (k <= 2^28)
-    int m, n, groups, n_tiles;
+    int m, n, groups;
+    int nt0, n_tiles;        // this launch's tiles of output channels
     int x_total, y_total;    // rows of x and y: an index outside them is no row
     int act, y_type;
 };
@@ -196,7 +197,7 @@ __device__ __forceinline__ Tile find_tile(const LinearArgs &a) {
     }
     const int band = (int)(id / ((long)BAND * a.n_tiles));
     const int rest = (int)(id - (long)band * BAND * a.n_tiles), bh = min(BAND, tiles_g - band * BAND);
-    t.nt = rest / bh;
+    t.nt = a.nt0 + rest / bh;
     t.r0 = lo_g + (band * BAND + rest % bh) * BM;
     t.r1 = t.r0 < lo_g ? t.r0 : min(t.r0 + BM, hi_g);  // offsets that do not ascend may count more tiles than an int holds: none then
     return t;
