@@ -462,6 +462,12 @@ int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_
                       const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
                       void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k);
 
+/* Which kernel form a product of these sizes takes, for tests and profiles (host only; no GPU is needed): few rows with k split over waves,
+ * 0: 16 x 16 outputs per workgroup, 1: 32 x 16, 2: 32 x 32; tiles through LDS, 3: 64 x 64, 4: 128 x 128, 5: 128 x 128 with waves of 64 x 64,
+ * 6: 256 x 256.  groups = 0: without offsets (pb_linear_i8).  align: the bytes, a power of two up to 16, on which every row of x and w starts.
+ * The rule may change with a release. */
+int pb_linear_form(int type, uint64_t m, uint32_t n, uint32_t k, uint32_t groups, uint32_t align, int *form);
+
 /* ======================================================================================
  *  utilities
  * ====================================================================================== */

@@ -51,7 +51,7 @@ SYMBOLS = [
     "pb_mlhash_image", "pb_embed_batch_images", "pb_embed_batch_images_device", "pb_embed_stage_acquire", "pb_embed_stage_release", "pb_embed_stage_close",
     "pb_embed_stage_commit", "pb_embed_stage_abort", "pb_resize_to_fill",
     "pb_embed_set_option", "pb_pinned_alloc", "pb_pinned_free", "pb_embed_tune_ms", "pb_embed_get_tuning", "pb_embed_set_tuning", "pb_fill_synthetic", "pb_fill_synthetic_images", "pb_fill_synthetic_scenes",
-    "pb_quantize_rows", "pb_linear_i8", "pb_group_rows", "pb_linear_grouped",
+    "pb_quantize_rows", "pb_linear_i8", "pb_group_rows", "pb_linear_grouped", "pb_linear_form",
     "pb_phash_create", "pb_phash_destroy", "pb_phash_image", "pb_phash_batch_images", "pb_phash_small_image",
 ]
 
@@ -161,6 +161,7 @@ def lib():
         L.pb_linear_i8.argtypes = [C.c_int, vp, vp, u64, vp, vp, u64, vp, vp, C.c_int, vp, C.c_int, u64, u64, u32, u32]
         L.pb_group_rows.argtypes = [C.c_int, vp, vp, u64, u32, vp, vp]
         L.pb_linear_grouped.argtypes = [C.c_int, vp, C.c_int, vp, u64, u64, vp, vp, u64, vp, vp, vp, u32, vp, vp, C.c_int, vp, C.c_int, u64, u64, u64, u32, u32]
+        L.pb_linear_form.argtypes = [C.c_int, u64, u32, u32, u32, u32, C.POINTER(C.c_int)]
         _lib = L
     return _lib
 
@@ -178,6 +179,13 @@ def device_count() -> int:
     n = C.c_int(0)
     rc = lib().pb_device_count(C.byref(n))
     return n.value if rc == PB_OK else 0
+
+
+def linear_form(type_: int, m: int, n: int, k: int, groups: int = 0, align: int = 16) -> int:
+    """the kernel form (0 .. 6, pb_linear_form) of a product of these sizes"""
+    form = C.c_int(-1)
+    _check(lib().pb_linear_form(type_, m, n, k, groups, align, C.byref(form)))
+    return form.value
 
 
 def topk_merge(ids: np.ndarray, dist: np.ndarray, counts: np.ndarray, k: int):

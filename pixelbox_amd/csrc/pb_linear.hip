@@ -291,6 +291,24 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
     return PB_OK;
 }
 
+int pb_linear_form(int type, uint64_t m, uint32_t n, uint32_t k, uint32_t groups, uint32_t align, int *form) {
+    const char *who = "pb_linear_form";
+    PB_CHECK(type == PB_TYPE_I8 || !bad_type(type), PB_ERR_INVALID, "%s: unknown type %d", who, type);
+    PB_CHECK(m >= 1 && m <= MAX_ROWS && n >= 1 && n <= (uint32_t)INT_MAX / 2 && k <= 1u << 28 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID,
+             "%s: m = %llu, n = %u, k = %u, groups = %u is out of range", who, (unsigned long long)m, n, k, groups);
+    PB_CHECK(align >= 1 && align <= 16 && (align & (align - 1)) == 0 && form, PB_ERR_INVALID, "%s: align = %u (1, 2, 4, 8, 16), or no room for the form", who, align);
+    LinearArgs a = {};
+    const int32_t some = 0;
+    a.offsets = groups ? &some : nullptr;  // never followed
+    a.kb = (int)k * type_bytes(type);
+    a.m = (int)m;
+    a.n = (int)n;
+    a.groups = groups ? (int)groups : 1;
+    *form = pick_form(a, type == PB_TYPE_F32, align == 16 ? 16 : align >= 4 || type == PB_TYPE_F32 ? 4 : 1);
+    PB_CHECK(*form != FORMS, PB_ERR_INVALID, "%s: %d x %d is more than one launch takes", who, a.m, a.n);
+    return PB_OK;
+}
+
 int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
                       const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,
                       void *y, int y_type, uint64_t y_total, uint64_t ldy, uint64_t m, uint32_t n, uint32_t k) {
