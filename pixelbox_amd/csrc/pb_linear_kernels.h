@@ -279,9 +279,21 @@ template <int T, int W> struct Chan {
     __device__ __forceinline__ void finish(const LinearArgs &a, const typename Acc<T>::e (&s)[W], float row_scale, int yr, int c0) const {
         float v[W];
 #pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = (float)s[i];
+        if constexpr (T == I8) {
+            // the sum times the row's scale leaves the range of f32 where the result need not: rows of values beyond 10^31 (a sum has up to 31
+            // bits), and scales near the smallest ones.  There a power of two is taken out and put back
+            if (row_scale >= 0x1p-100f && row_scale <= 0x1p96f) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = v[i] * row_scale * scale[i];
+            } else {
+                const float out = row_scale > 1.0f ? 0x1p-64f : 0x1p64f, back = row_scale > 1.0f ? 0x1p64f : 0x1p-64f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) v[i] = v[i] * (row_scale * out) * scale[i] * back;
+            }
+        }
+#pragma unroll
         for (int i = 0; i < W; ++i) {
-            v[i] = (float)s[i];
-            if constexpr (T == I8) v[i] = v[i] * row_scale * scale[i];
             v[i] += bias[i];
             if constexpr (!PLAIN) v[i] = act_f(v[i], a.act);
         }
