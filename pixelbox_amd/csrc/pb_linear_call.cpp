@@ -2,7 +2,7 @@
 //
 // One such call is a kernel of a few microseconds; checking a dozen tensor properties from Python and converting sixteen arguments
 // through ctypes takes as long again (1 x 256 x 1280 in 8 bits, two calls: 14.3 us).  This module looks at the usual call -- right
-// types, shapes and devices, contiguous tensors, no gradients -- and makes it; whatever it does not recognise it leaves alone (None), for
+// types, shapes and devices, contiguous tensors, no gradients or tangents -- and makes it; whatever it does not recognise it leaves alone (None), for
 // pixelbox_amd/linear.py to check in full, to name the error or to make the call itself.  The library's functions are handed over by
 // address (bind), so that this module uses the same copy of it as everything else in the process.
 #define PY_SSIZE_T_CLEAN
@@ -27,7 +27,7 @@ const Tensor *tensor(PyObject *o) { return THPVariable_CheckExact(o) ? &THPVaria
 
 bool usual(const Tensor *t, at::ScalarType type, int device, int dims) {
     return t && t->scalar_type() == type && t->is_cuda() && t->get_device() == device && t->dim() == dims && t->layout() == at::kStrided && t->is_contiguous() &&
-           !(t->requires_grad() && at::GradMode::is_enabled());
+           !(t->requires_grad() && at::GradMode::is_enabled()) && !t->_fw_grad(/*level=*/0).defined();
 }
 bool vector(const Tensor *t, at::ScalarType type, int device, int64_t n) { return usual(t, type, device, 1) && t->size(0) == n; }
 bool matrix(const Tensor *t, at::ScalarType type, int device, int64_t m, int64_t n) { return usual(t, type, device, 2) && t->size(0) == m && t->size(1) == n; }

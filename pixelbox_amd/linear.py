@@ -11,14 +11,15 @@ strides and devices are checked here, the work is queued on the tensors' device 
     y = linear_grouped(features, weights, offsets, rows=order, bias=bias, act="tanh")   # weights [heads, n, k]
 
 Rows may have any stride >= their length (a slice of a wider tensor), the last axis is contiguous; an output overlaps no other
-tensor of its call.  Products have no gradient: an operand that requires one is refused, and an output that a backward pass has
-saved is counted as written.
+tensor of its call.  Products have no derivative, backward or forward: an operand that requires a gradient or carries a tangent is
+refused, and an output that a backward pass has saved is counted as written.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import capi
 
@@ -87,12 +88,14 @@ def _ld(t: torch.Tensor, name: str) -> int:
 
 
 def _no_grad(*tensors) -> None:
-    if not torch.is_grad_enabled():
-        return
+    grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is None or not t.requires_grad:
+        if t is None:
             continue
-        raise ValueError("these products have no gradient: an operand requires one (detach it, or call under torch.no_grad())")
+        if grad and t.requires_grad:
+            raise ValueError("these products have no gradient: an operand requires one (detach it, or call under torch.no_grad())")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError("these products have no derivative: an operand has a tangent (torch.autograd.forward_ad.unpack_dual gives its values alone)")
 
 
 def _written(*tensors) -> None:
