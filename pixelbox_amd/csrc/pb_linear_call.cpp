@@ -27,7 +27,7 @@ const Tensor *tensor(PyObject *o) { return THPVariable_CheckExact(o) ? &THPVaria
 
 bool usual(const Tensor *t, at::ScalarType type, int device, int dims) {
     return t && t->scalar_type() == type && t->is_cuda() && t->get_device() == device && t->dim() == dims && t->layout() == at::kStrided && t->is_contiguous() &&
-           !(t->requires_grad() && at::GradMode::is_enabled()) && !t->_fw_grad(/*level=*/0).defined();
+           !(t->requires_grad() && at::GradMode::is_enabled()) && !t->is_neg() && !t->_is_zerotensor() && !t->_fw_grad(/*level=*/0).defined();
 }
 bool vector(const Tensor *t, at::ScalarType type, int device, int64_t n) { return usual(t, type, device, 1) && t->size(0) == n; }
 bool matrix(const Tensor *t, at::ScalarType type, int device, int64_t m, int64_t n) { return usual(t, type, device, 2) && t->size(0) == m && t->size(1) == n; }

@@ -12,7 +12,7 @@ strides and devices are checked here, the work is queued on the tensors' device 
 
 Rows may have any stride >= their length (a slice of a wider tensor), the last axis is contiguous; an output overlaps no other
 tensor of its call.  Products have no derivative, backward or forward: an operand that requires a gradient or carries a tangent is
-refused, and an output that a backward pass has saved is counted as written.
+refused, and an output that a backward pass has saved is counted as written.  Negated views are refused too.
 """
 from __future__ import annotations
 
@@ -63,7 +63,9 @@ def _load():
 
 
 def _check(t: torch.Tensor, name: str, shape: tuple, dtypes: tuple, index: int) -> None:
-    """dtype, device, shape (None: any length) and a contiguous last axis"""
+    """dtype, device, shape (None: any length), a contiguous last axis and values that are what lies in memory"""
+    if t.is_neg():  # a view whose values are the memory's with the other sign
+        raise ValueError(f"{name} is a negated view (resolve_neg() gives a tensor of its own)")
     if t.dtype in dtypes and t.get_device() == index and t.shape == shape and t.is_contiguous():
         return
     if t.dtype not in dtypes:

@@ -1,4 +1,4 @@
-"""The compiled short way leaves operands with tangents alone, and they are refused behind it."""
+"""The compiled short way leaves operands with tangents and negated views alone, and they are refused behind it."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -40,3 +40,20 @@ def test_tangents():
         # the values alone
         y = linear.linear_grouped(forward_ad.unpack_dual(dual(x)).primal, w, offsets)
         assert (y == 32).all()
+
+
+def test_negated_views():
+    short = linear._load()
+    ok = i8(1, 1)
+    minus = torch.ones(1, dtype=torch.complex64, device="cuda").conj().imag
+    assert minus.is_neg() and minus.is_contiguous()
+    assert short.linear_i8(*ok) == 0
+    for i in (1, 3, 4):
+        assert short.linear_i8(*ok[:i], minus, *ok[i + 1:]) is None, i
+    with pytest.raises(ValueError, match="x_scale is a negated view"):
+        linear.linear_i8(ok[0], minus, *ok[2:4], out=ok[6])
+    column = torch.ones((6, 1), dtype=torch.complex64, device="cuda").conj().imag
+    with pytest.raises(ValueError, match="x is a negated view"):
+        linear.quantize_rows(column)
+    c, s = linear.quantize_rows(column.resolve_neg())
+    assert (c == 0).all()  # the imaginary part of 1
