@@ -419,7 +419,8 @@ int pb_phash_small_image(pb_phasher *p, const uint8_t *rgb, uint32_t width, uint
  *  and inside a graph capture.  m = 0 (and n = 0) is a call that does nothing.
  *  ld* is the distance between rows in ELEMENTS; any value >= the row length, any alignment of a row to its type.  Rows on 16 bytes
  *  run fastest, rows off 4 bytes (an odd k of 8- or 16-bit values without padding) slowest: about half as fast where the product
- *  fills the GPU.  Rows number less than 2^31 - 256; no output may overlap an input or another output.
+ *  fills the GPU.  Rows number less than 2^31 - 256; no output may share a byte with an input or another
+ *  output (column ranges of one wider buffer, at one row stride in bytes, do not; at different strides spans that meet are refused).
  * ====================================================================================== */
 #define PB_TYPE_F32 0
 #define PB_TYPE_BF16 1

@@ -31,12 +31,23 @@ struct Device {
     }
 };
 
-bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+// rows of `len` bytes, `pitch` bytes apart
+struct Rows {
+    const void *p;
+    uint64_t rows, pitch, len;
+};
+Rows rows_of(const void *p, uint64_t rows, uint64_t ld, uint64_t n, int size) { return {p, rows, ld * size, n * size}; }
+Rows vector_of(const void *p, uint64_t n) { return {p, 1, n * 4, n * 4}; }
+// whether some byte may be in both: exact for rows at one pitch (column ranges of one wider tensor are apart), and for a single row
+// between others; rows at different pitches count as one where the spans from first to last byte meet
+bool overlap(const Rows &a, const Rows &b) {
+    if (!a.p || !b.p || !a.rows || !b.rows || !a.len || !b.len) return false;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    if (x >= y + (b.rows - 1) * b.pitch + b.len || y >= x + (a.rows - 1) * a.pitch + a.len) return false;
+    if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+    const uint64_t pitch = a.rows > 1 ? a.pitch : b.pitch, d = y >= x ? (y - x) % pitch : (pitch - (x - y) % pitch) % pitch;
+    return d < a.len || d + b.len > pitch;
 }
-// bytes from the first row to the end of the last one
-uint64_t extent(uint64_t rows, uint64_t ld, uint64_t n, int size) { return rows && n ? ((rows - 1) * ld + n) * size : 0; }
 bool bad_type(int t) { return t != PB_TYPE_F32 && t != PB_TYPE_BF16 && t != PB_TYPE_F16; }
 bool misaligned(const void *p, int size) { return ((uintptr_t)p & (uintptr_t)(size - 1)) != 0; }
 
@@ -177,12 +188,11 @@ int linear(const char *who, int device, void *stream, int type, const void *x, u
     PB_CHECK(!misaligned(x_scale, 4) && !misaligned(w_scale, 4) && !misaligned(bias, 4) && !misaligned(offsets, 4) && !misaligned(x_rows, 4) &&
                  !misaligned(y_rows, 4),
              PB_ERR_INVALID, "%s: a scale, bias or index array is not aligned to 4 bytes", who);
-    const uint64_t y_bytes = extent(y_total, ldy, n, y_size);
-    PB_CHECK(!overlap(y, y_bytes, x, extent(x_total, ldx, k, size)) && !overlap(y, y_bytes, w, extent((uint64_t)groups * n, ldw, k, size)), PB_ERR_INVALID,
-             "%s: y overlaps an operand", who);
-    PB_CHECK(!(i8 && (overlap(y, y_bytes, x_scale, x_total * 4) || overlap(y, y_bytes, w_scale, (uint64_t)groups * n * 4))) &&
-                 !overlap(y, y_bytes, bias, (uint64_t)groups * n * 4) && !overlap(y, y_bytes, offsets, (groups + 1ull) * 4) &&
-                 !overlap(y, y_bytes, x_rows, m * 4) && !overlap(y, y_bytes, y_rows, m * 4),
+    const Rows ys = rows_of(y, y_total, ldy, n, y_size);
+    const uint64_t channels = (uint64_t)groups * n;
+    PB_CHECK(!overlap(ys, rows_of(x, x_total, ldx, k, size)) && !overlap(ys, rows_of(w, channels, ldw, k, size)), PB_ERR_INVALID, "%s: y overlaps an operand", who);
+    PB_CHECK(!(i8 && (overlap(ys, vector_of(x_scale, x_total)) || overlap(ys, vector_of(w_scale, channels)))) && !overlap(ys, vector_of(bias, channels)) &&
+                 !overlap(ys, vector_of(offsets, groups + 1ull)) && !overlap(ys, vector_of(x_rows, m)) && !overlap(ys, vector_of(y_rows, m)),
              PB_ERR_INVALID, "%s: y overlaps a scale, the bias or an index array", who);
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
@@ -253,8 +263,8 @@ int pb_quantize_rows(int device, void *stream, const void *x, int x_type, uint64
     const int size = type_bytes(x_type);
     PB_CHECK(scale && (k == 0 || (x && codes)), PB_ERR_INVALID, "%s: null buffer", who);
     PB_CHECK(!misaligned(x, size) && !misaligned(scale, 4), PB_ERR_INVALID, "%s: a buffer is not aligned to its type", who);
-    const uint64_t xb = extent(m, ldx, k, size), cb = extent(m, ldc, k, 1);
-    PB_CHECK(!overlap(codes, cb, x, xb) && !overlap(scale, m * 4, x, xb) && !overlap(scale, m * 4, codes, cb), PB_ERR_INVALID, "%s: buffers overlap", who);
+    const Rows xr = rows_of(x, m, ldx, k, size), cr = rows_of(codes, m, ldc, k, 1), sr = vector_of(scale, m);
+    PB_CHECK(!overlap(cr, xr) && !overlap(sr, xr) && !overlap(sr, cr), PB_ERR_INVALID, "%s: buffers overlap", who);
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -279,8 +289,8 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
     PB_CHECK(groups >= 1 && groups <= PB_MAX_GROUPS, PB_ERR_INVALID, "%s: groups = %u (1 .. %u)", who, groups, PB_MAX_GROUPS);
     PB_CHECK(offsets && (m == 0 || (group && order)), PB_ERR_INVALID, "%s: null buffer", who);
     PB_CHECK(!misaligned(group, 4) && !misaligned(offsets, 4) && !misaligned(order, 4), PB_ERR_INVALID, "%s: a buffer is not aligned to 4 bytes", who);
-    PB_CHECK(!overlap(group, m * 4, order, m * 4) && !overlap(group, m * 4, offsets, (groups + 1ull) * 4) && !overlap(order, m * 4, offsets, (groups + 1ull) * 4),
-             PB_ERR_INVALID, "%s: buffers overlap", who);
+    const Rows gr = vector_of(group, m), orr = vector_of(order, m), fr = vector_of(offsets, groups + 1ull);
+    PB_CHECK(!overlap(gr, orr) && !overlap(gr, fr) && !overlap(orr, fr), PB_ERR_INVALID, "%s: buffers overlap", who);
     Device dev(device);
     PB_CHECK(dev.ok, PB_ERR_HIP, "%s: no HIP device %d", who, device);
     const int vec = !misaligned(group, 16);
