@@ -1956,6 +1956,19 @@ static int forward_features(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, fl
     return rc;
 }
 
+// the end of a call that has queued its work with the status rc: nothing of a call that failed half-way is left running, and its batch's
+// range flag is not reported by a later call
+static int finish_call(pb_embedder *e, int rc) {
+    if (e->opt_async) return rc;
+    const hipError_t waited = hipStreamSynchronize(e->stream);
+    if (rc) {
+        if (e->h_range) __atomic_store_n(e->h_range, 0u, __ATOMIC_RELEASE);
+        return rc;
+    }
+    PB_HIP(waited);
+    return range_status(e);
+}
+
 int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, float *d_features) {
     PB_CHECK(e, PB_ERR_INVALID, "pb_embed_features_device: null embedder");
     PB_CHECK(n <= e->max_batch, PB_ERR_INVALID, "pb_embed_features_device: n = %u > max_batch %u", n, e->max_batch);
@@ -1967,10 +1980,7 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
     if (n == 0) return PB_OK;
     std::lock_guard<std::mutex> lock(e->mu);
     pb::DeviceGuard guard(e->device);
-    const int rc = forward_features(e, d_rgb, n, d_features);
-    if (rc || e->opt_async) return rc;
-    PB_HIP(hipStreamSynchronize(e->stream));
-    return range_status(e);
+    return finish_call(e, forward_features(e, d_rgb, n, d_features));
 }
 
 int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
@@ -1982,10 +1992,19 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
     PB_CHECK(d >= 1 && d <= (1u << 20), PB_ERR_INVALID, "pb_embed_heads_device: d = %u (1 .. 2^20)", d);
     PB_CHECK(n == 0 || (d_rgb && d_w && d_head && (d_out_u8 || d_out_f32) && (type != PB_TYPE_I8 || d_w_scale)), PB_ERR_INVALID,
              "pb_embed_heads_device: null buffer");
-    const auto apart = [](const void *p, uint64_t pb, const void *q, uint64_t qb) { return !p || !q || (uintptr_t)p + pb <= (uintptr_t)q || (uintptr_t)q + qb <= (uintptr_t)p; };
-    PB_CHECK(apart(d_out_u8, (uint64_t)n * d, d_out_f32, (uint64_t)n * d * 4) && apart(d_out_u8, (uint64_t)n * d, d_head, (uint64_t)n * 4) &&
-                 apart(d_out_f32, (uint64_t)n * d * 4, d_head, (uint64_t)n * 4),
-             PB_ERR_INVALID, "pb_embed_heads_device: outputs overlap each other or d_head");
+    const auto off4 = [](const void *p) { return ((uintptr_t)p & 3) != 0; };
+    PB_CHECK(!(type == PB_TYPE_F32 && off4(d_w)) && !off4(d_w_scale) && !off4(d_bias) && !off4(d_head) && !off4(d_out_f32), PB_ERR_INVALID,
+             "pb_embed_heads_device: a buffer is not aligned to its type");
+    const uint64_t out = (uint64_t)n * d, channels = (uint64_t)heads * d;
+    const auto apart = [&](const void *p, uint64_t bytes) {  // from both outputs
+        const uintptr_t q = (uintptr_t)p, u8 = (uintptr_t)d_out_u8, f32 = (uintptr_t)d_out_f32;
+        return !p || ((!u8 || u8 + out <= q || q + bytes <= u8) && (!f32 || f32 + 4 * out <= q || q + bytes <= f32));
+    };
+    PB_CHECK(!d_out_u8 || !d_out_f32 || (uintptr_t)d_out_u8 + out <= (uintptr_t)d_out_f32 || (uintptr_t)d_out_f32 + 4 * out <= (uintptr_t)d_out_u8, PB_ERR_INVALID,
+             "pb_embed_heads_device: the outputs overlap");
+    PB_CHECK(apart(d_w, channels * 1280 * (type == PB_TYPE_F32 ? 4 : 1)) && apart(type == PB_TYPE_I8 ? d_w_scale : nullptr, 4 * channels) &&
+                 apart(d_bias, 4 * channels) && apart(d_head, 4ull * n),
+             PB_ERR_INVALID, "pb_embed_heads_device: an output overlaps the weights, their scales, the bias or d_head");
     if (n == 0) return PB_OK;
     std::lock_guard<std::mutex> lock(e->mu);
     pb::DeviceGuard guard(e->device);
@@ -2007,21 +2026,23 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
         }
         val = e->hd_val;
     }
-    if ((rc = forward_features(e, d_rgb, n, e->hd_feat))) return rc;
-    if ((rc = pb_group_rows(e->device, e->stream, d_head, n, heads, e->hd_offsets, e->hd_order))) return rc;
-    const void *x = e->hd_feat;
-    if (type == PB_TYPE_I8) {
-        if ((rc = pb_quantize_rows(e->device, e->stream, e->hd_feat, PB_TYPE_F32, n, 1280, 1280, e->hd_codes, 1280, e->hd_scale))) return rc;
-        x = e->hd_codes;
-    }
-    if ((rc = pb::linear_heads(e->device, e->stream, type, x, e->hd_scale, d_w, d_w_scale, d_bias, e->hd_offsets, heads, e->hd_order, val, n, d, 1280))) return rc;
-    if (d_out_u8) {
-        hipLaunchKernelGGL(k_hash_rows, dim3((d + 255) / 256, n), dim3(256), 0, e->stream, val, d_head, (int)heads, (int)d, d_out_u8);
-        PB_HIP(hipGetLastError());
-    }
-    if (e->opt_async) return PB_OK;
-    PB_HIP(hipStreamSynchronize(e->stream));
-    return range_status(e);
+    const auto queue = [&]() -> int {
+        int rc = forward_features(e, d_rgb, n, e->hd_feat);
+        if (rc) return rc;
+        if ((rc = pb_group_rows(e->device, e->stream, d_head, n, heads, e->hd_offsets, e->hd_order))) return rc;
+        const void *x = e->hd_feat;
+        if (type == PB_TYPE_I8) {
+            if ((rc = pb_quantize_rows(e->device, e->stream, e->hd_feat, PB_TYPE_F32, n, 1280, 1280, e->hd_codes, 1280, e->hd_scale))) return rc;
+            x = e->hd_codes;
+        }
+        if ((rc = pb::linear_heads(e->device, e->stream, type, x, e->hd_scale, d_w, d_w_scale, d_bias, e->hd_offsets, heads, e->hd_order, val, n, d, 1280))) return rc;
+        if (d_out_u8) {
+            hipLaunchKernelGGL(k_hash_rows, dim3((d + 255) / 256, n), dim3(256), 0, e->stream, val, d_head, (int)heads, (int)d, d_out_u8);
+            PB_HIP(hipGetLastError());
+        }
+        return PB_OK;
+    };
+    return finish_call(e, queue());
 }
 
 int pb_embed_check_range(pb_embedder *e) {
