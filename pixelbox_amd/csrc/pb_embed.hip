@@ -81,6 +81,7 @@ struct pb_embedder {
     float *feat_dst = nullptr;
     float *hd_feat = nullptr, *hd_scale = nullptr, *hd_val = nullptr;
     size_t hd_val_cap = 0;
+    bool hd_val_queued = false;  // a queued call has used hd_val
     int *hd_order = nullptr, *hd_offsets = nullptr;
     int8_t *hd_codes = nullptr;
     long long *buf_part = nullptr;  // SE pooling partial sums, 2^-24 fixed point; buf_part[-1] holds the address of *h_range (se_range_check)
@@ -1983,6 +1984,33 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
     return finish_call(e, forward_features(e, d_rgb, n, d_features));
 }
 
+// room for the values of n images of d channels where the caller takes the bytes alone: n rounded up to a power of two, or n itself if
+// there is not that much memory.  A smaller buffer is given back, unless a queued call has used it: it may be at work, or part of a graph
+static int heads_values(pb_embedder *e, uint32_t n, uint32_t d) {
+    const size_t need = (size_t)n * d;
+    if (e->hd_val_cap >= need) return PB_OK;
+    if (e->hd_val && !e->hd_val_queued) {
+        e->allocs.erase(std::find(e->allocs.begin(), e->allocs.end(), (void *)e->hd_val));
+        (void)hipFree(e->hd_val);
+    }
+    e->hd_val = nullptr;
+    e->hd_val_cap = 0;
+    e->hd_val_queued = false;
+    size_t rows = 1;
+    while (rows < n) rows *= 2;
+    for (const size_t cap : {std::min<size_t>(rows, e->max_batch) * d, need}) {
+        void *q = nullptr;
+        if (hipMalloc(&q, cap * sizeof(float)) == hipSuccess) {
+            e->allocs.push_back(q);
+            e->hd_val = static_cast<float *>(q);
+            e->hd_val_cap = cap;
+            return PB_OK;
+        }
+        (void)hipGetLastError();  // reported here, not by the next launch
+    }
+    return pb::fail(PB_ERR_HIP, "pb_embed_heads_device: no memory for %zu values", need);
+}
+
 int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
                           uint32_t heads, uint32_t d, const int *d_head, uint8_t *d_out_u8, float *d_out_f32) {
     PB_CHECK(e, PB_ERR_INVALID, "pb_embed_heads_device: null embedder");
@@ -2019,12 +2047,9 @@ int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int 
     }
     float *val = d_out_f32;
     if (!val) {
-        if (e->hd_val_cap < B * d) {  // wider heads than any before; the smaller buffer stays, for what is queued or captured with it
-            const size_t cap = std::max(B * d, 2 * e->hd_val_cap);
-            if ((rc = dalloc(e, &e->hd_val, cap))) return rc;
-            e->hd_val_cap = cap;
-        }
+        if ((rc = heads_values(e, n, d))) return rc;
         val = e->hd_val;
+        e->hd_val_queued |= e->opt_async;
     }
     const auto queue = [&]() -> int {
         int rc = forward_features(e, d_rgb, n, e->hd_feat);
