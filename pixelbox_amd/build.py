@@ -34,6 +34,7 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=o
 # the short way from torch tensors to the linear layers' entry points (pixelbox_amd/linear.py): host code, against torch's headers
 CALL_SRC = "pb_linear_call.cpp"
 CALL_LIB = os.path.join(HERE, "_linear_call.so")
+CALL_STAMP = CALL_LIB + ".stamp"
 # RCCL (the sharded index's all-gather, pb_sharded.hip) is dlopen'ed at pb_sharded_create: a single-GPU host never loads it
 LINK = ["-ldl"]
 
@@ -52,7 +53,7 @@ def _extra() -> list[str]:
 def source_hash() -> str:
     h = hashlib.sha256()
     h.update(" ".join(FLAGS + _extra() + LINK).encode())
-    for rel in SOURCES + HEADERS + [CALL_SRC]:
+    for rel in SOURCES + HEADERS:
         p = os.path.join(CSRC, rel)
         if os.path.exists(p):
             h.update(rel.encode())
@@ -66,11 +67,25 @@ def _torch_dir() -> str | None:
     return os.path.dirname(spec.origin) if spec and spec.origin else None
 
 
+def _stamp(path: str) -> str:
+    if not os.path.exists(path):
+        return ""
+    with open(path) as f:
+        return f.read().strip()
+
+
+def _needs_lib() -> bool:
+    return not os.path.exists(LIB) or _stamp(STAMP) != source_hash()
+
+
+def _needs_call() -> bool:
+    """whether _linear_call.so is to be tried: not where it was tried with the same sources and could not be built"""
+    want = call_hash()
+    return bool(want) and not (_stamp(CALL_STAMP) == want and os.path.exists(CALL_LIB)) and _stamp(CALL_STAMP) != "failed " + want
+
+
 def needs_build() -> bool:
-    if not (os.path.exists(LIB) and os.path.exists(STAMP)) or (_torch_dir() and not os.path.exists(CALL_LIB)):
-        return True
-    with open(STAMP) as f:
-        return f.read().strip() != source_hash()
+    return _needs_lib() or _needs_call()
 
 
 def _compile(src: str, verbose: bool) -> str:
@@ -82,39 +97,75 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
-def _build_call(verbose: bool) -> bool:
-    """_linear_call.so; False where there is no torch to build it against (a host without Python has no use for it)"""
+def _call_command() -> list[str]:
+    """what compiles _linear_call.so; empty where there is no torch to build it against (a host without Python has no use for it)"""
     t = _torch_dir()
     if t is None:
+        return []
+    hipcc = shutil.which("hipcc")
+    rocm = os.environ.get("ROCM_PATH") or (os.path.dirname(os.path.dirname(os.path.realpath(hipcc))) if hipcc else "/opt/rocm")
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-I" + os.path.join(t, "include"),
+            "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"), "-I" + sysconfig.get_paths()["include"],
+            os.path.join(CSRC, CALL_SRC), "-o", CALL_LIB, "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
+            "-Wl,-rpath," + os.path.join(t, "lib")]
+
+
+def call_hash() -> str:
+    cmd = _call_command()
+    if not cmd:
+        return ""
+    h = hashlib.sha256(" ".join(cmd).encode())
+    for rel in (CALL_SRC, os.path.join("..", "..", "include", "pixelbox_hip.h")):
+        with open(os.path.join(CSRC, rel), "rb") as f:
+            h.update(f.read())
+    return h.hexdigest()
+
+
+def _build_call(verbose: bool) -> bool:
+    """_linear_call.so.  It only shortens calls that pixelbox_amd/linear.py makes without it too: where it cannot be built (no headers, another
+    compiler, a torch without HIP) that is said, an older one is taken away, and the library is built all the same."""
+    cmd, want = _call_command(), call_hash()
+    if not cmd:
         return False
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-I" + os.path.join(t, "include"),
-           "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I/opt/rocm/include", "-I" + sysconfig.get_paths()["include"],
-           os.path.join(CSRC, CALL_SRC), "-o", CALL_LIB, "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
-           "-Wl,-rpath," + os.path.join(t, "lib")]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
-    subprocess.check_call(cmd)
-    return True
+    try:
+        subprocess.check_call(cmd)
+    except (OSError, subprocess.CalledProcessError) as e:
+        print(f"pixelbox_amd.build: {os.path.basename(CALL_LIB)} could not be built ({e}); calls from torch take the longer way", file=sys.stderr)
+        if os.path.exists(CALL_LIB):
+            os.remove(CALL_LIB)
+        want = "failed " + want
+    with open(CALL_STAMP, "w") as f:
+        f.write(want + "\n")
+    return not want.startswith("failed")
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    want = source_hash()
-    if not force and not needs_build():
-        print(f"pixelbox_amd.build: {os.path.basename(LIB)} is up to date with the sources (sha256 {want[:16]})", file=sys.stderr)
-        return LIB
+def _build_lib(verbose: bool) -> int:
     srcs = [os.path.join(CSRC, s) for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
+    want = source_hash()
     with ThreadPoolExecutor(max_workers=min(5, len(srcs))) as ex:
-        call = ex.submit(_build_call, verbose)
         objs = list(ex.map(lambda s: _compile(s, verbose), srcs))
-        has_call = call.result()
     cmd = [_hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs + LINK
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.check_call(cmd)
     with open(STAMP, "w") as f:
         f.write(want + "\n")
-    print(f"pixelbox_amd.build: compiled {len(srcs)} translation units for gfx950 -> {os.path.basename(LIB)} "
-          f"{'and _linear_call.so ' if has_call else ''}(sha256 of sources + flags {want[:16]})", file=sys.stderr)
+    return len(srcs)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    lib, call = force or _needs_lib(), force or _needs_call()
+    with ThreadPoolExecutor(max_workers=1) as ex:  # beside the library's translation units
+        beside = ex.submit(_build_call, verbose) if call else None
+        n = _build_lib(verbose) if lib else 0
+        has_call = beside.result() if beside else os.path.exists(CALL_LIB)
+    if not lib and not call:
+        print(f"pixelbox_amd.build: {os.path.basename(LIB)} is up to date with the sources (sha256 {_stamp(STAMP)[:16]})", file=sys.stderr)
+    else:
+        print(f"pixelbox_amd.build: compiled {n} translation units for gfx950 -> {os.path.basename(LIB)} "
+              f"{'and _linear_call.so ' if has_call else ''}(sha256 of sources + flags {_stamp(STAMP)[:16]})", file=sys.stderr)
     return LIB
 
 
