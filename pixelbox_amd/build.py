@@ -14,6 +14,7 @@ from __future__ import annotations
 import hashlib
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -97,6 +98,16 @@ def _compile(src: str, verbose: bool) -> str:
     return obj
 
 
+def call_tag() -> str:
+    """the torch and the Python whose layouts _linear_call.so has compiled in"""
+    t, version = _torch_dir(), ""
+    if t is not None:
+        with open(os.path.join(t, "version.py")) as f:
+            found = re.search(r"^__version__\s*=\s*['\"]([^'\"]+)", f.read(), re.M)
+        version = found.group(1) if found else "unknown"
+    return f"torch {version} {sysconfig.get_config_var('SOABI')}"
+
+
 def _call_command() -> list[str]:
     """what compiles _linear_call.so; empty where there is no torch to build it against (a host without Python has no use for it)"""
     t = _torch_dir()
@@ -104,7 +115,8 @@ def _call_command() -> list[str]:
         return []
     hipcc = shutil.which("hipcc")
     rocm = os.environ.get("ROCM_PATH") or (os.path.dirname(os.path.dirname(os.path.realpath(hipcc))) if hipcc else "/opt/rocm")
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", "-I" + os.path.join(t, "include"),
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f'-DPB_BUILT_FOR="{call_tag()}"',
+            "-I" + os.path.join(t, "include"),
             "-I" + os.path.join(t, "include", "torch", "csrc", "api", "include"), "-I" + os.path.join(rocm, "include"), "-I" + sysconfig.get_paths()["include"],
             os.path.join(CSRC, CALL_SRC), "-o", CALL_LIB, "-L" + os.path.join(t, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
             "-Wl,-rpath," + os.path.join(t, "lib")]

@@ -163,4 +163,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_linear_call", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__linear_call() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__linear_call() {
+    PyObject *m = PyModule_Create(&module);
+    // torch's and Python's layouts are compiled in: linear.py takes this module only where they are the running ones
+    if (m && PyModule_AddStringConstant(m, "built_for", PB_BUILT_FOR) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -17,6 +17,8 @@ refused, and an output that a backward pass has saved is counted as written.  Ne
 from __future__ import annotations
 
 import ctypes as C
+import sysconfig
+import warnings
 
 import torch
 from torch.autograd import forward_ad
@@ -49,16 +51,27 @@ def _device(t: torch.Tensor, name: str) -> int:
 _compiled = None
 
 
+def _usable(module):
+    """the module if it was built for the running torch and Python, whose layouts it has compiled in; else False"""
+    here = f"torch {torch.__version__} {sysconfig.get_config_var('SOABI')}"
+    built = getattr(module, "built_for", "an unknown torch")
+    if built == here:
+        return module
+    warnings.warn(f"pixelbox_amd: _linear_call.so was built for {built}, this is {here}: calls take the longer way until it is built again")
+    return False
+
+
 def _load():
     global _compiled
     L = capi.lib()
     try:
         from . import _linear_call
-    except ImportError:  # built without torch's headers: the calls below do the same
+    except ImportError:  # not built: the calls below do the same
         _compiled = False
     else:
-        _linear_call.bind(*(C.cast(f, C.c_void_p).value for f in (L.pb_quantize_rows, L.pb_linear_i8, L.pb_group_rows, L.pb_linear_grouped)))
-        _compiled = _linear_call
+        _compiled = _usable(_linear_call)
+    if _compiled:
+        _compiled.bind(*(C.cast(f, C.c_void_p).value for f in (L.pb_quantize_rows, L.pb_linear_i8, L.pb_group_rows, L.pb_linear_grouped)))
     return _compiled
 
 

@@ -76,3 +76,29 @@ def test_a_missing_file_is_built_again(tree):
     os.remove(build.LIB)
     build.build()
     assert tree.ran == ["host", "hipcc"]
+
+
+def test_another_torch_builds_it_again_and_nothing_else(tree, tmp_path, monkeypatch):
+    other = tmp_path / "torch"
+    other.mkdir()
+    (other / "version.py").write_text("__version__ = '9.9.1+rocm8.1'\ndebug = False\n")
+    build.build()
+    monkeypatch.setattr(build, "_torch_dir", lambda: str(other))
+    assert build.needs_build() and "9.9.1+rocm8.1" in build.call_tag()
+    tree.ran.clear()
+    build.build()
+    assert tree.ran == ["host"] and not build.needs_build()
+
+
+def test_a_module_built_for_another_torch_is_not_used():
+    from pixelbox_amd import linear
+
+    class Module:
+        built_for = build.call_tag()
+
+    assert linear._usable(Module) is Module  # what the build writes in is what the call looks for
+    Module.built_for = "torch 1.0.0 cpython-39-x86_64-linux-gnu"
+    with pytest.warns(UserWarning, match="built for torch 1.0.0"):
+        assert linear._usable(Module) is False
+    with pytest.warns(UserWarning, match="unknown"):
+        assert linear._usable(object()) is False
