@@ -897,8 +897,10 @@ __global__ __launch_bounds__(256) void k_quantize_rows(const uint8_t *__restrict
 
 // ---- k_group_rows ---------------------------------------------------------------------------------------------------------------------------
 // Workgroup g < groups counts the rows of smaller groups (its offset) and lists its own rows in ascending order; workgroup `groups`
-// lists the rows without a group behind all others.  Every workgroup reads the whole array (it sits in L2) instead of meeting the
-// others: no scratch memory, no atomics, one launch, one possible result.  A first walk, four consecutive rows per lane, turns each
+// lists the rows without a group behind all others.  Every workgroup reads the whole array instead of meeting the others: no scratch
+// memory, no atomics, one launch, one possible result.  The work is rows x (groups + 1): up to a million rows the array sits in each XCD's
+// L2 (4 MB), beyond that it comes from the cache behind them, and lists of more than one LDS map are read twice (131073 rows of 256 groups
+// 28 us, a million of 64 108, of 1024 417, 30 million of 1024 20 ms).  A first walk, four consecutive rows per lane, turns each
 // comparison into a lane mask: the counts come from the scalar unit's bit counts, the masks of matching rows go to LDS -- four
 // vector instructions for 64 rows, which is what bounds it (131072 rows, 256 groups: 27 us with a bit per lane put together by vector
 // instructions).  Then every lane takes words of 32 rows, learns by prefix sums over the bit counts where its rows go, and lists
