@@ -415,7 +415,7 @@ int pb_phash_small_image(pb_phasher *p, const uint8_t *rgb, uint32_t width, uint
  *  experts).
  *
  *  All pointers are DEVICE memory of `device`; `stream` is the hipStream_t the work is queued on (NULL: the device's null stream).
- *  A call checks its arguments, queues one kernel and returns: outputs are complete for later work on that stream, or once the
+ *  A call checks its arguments, queues one kernel (pb_quantize_rows several, from 8 million rows on) and returns: outputs are complete for later work on that stream, or once the
  *  caller has waited for it.  Nothing is allocated and no state outlives a call, so calls may run from any threads, on any streams,
  *  and inside a graph capture.  m = 0 (and n = 0) is a call that does nothing.
  *  ld* is the distance between rows in ELEMENTS; any value >= the row length, any alignment of a row to its type.  Rows on 16 bytes
@@ -458,8 +458,8 @@ int pb_group_rows(int device, void *stream, const int *group, uint64_t m, uint32
  * a row may differ from one batch to another) or i8 (as pb_linear_i8; x_scale f32[x_total] and w_scale f32[groups][n], ignored
  * for the others).  w: [groups][n][ldw], bias: f32[groups][n] or NULL.  With x_rows = y_rows = pb_group_rows' order, y is in the
  * order of x; with only x_rows the groups' results lie packed, as the input of a next layer that has only y_rows.  offsets
- * (int[groups + 1]) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,
- * a row number outside x ([0, x_total)) or y ([0, y_total)) is skipped.  A row of x may be listed any number of times, a row of y
+ * (int[groups + 1], ascending) and the row lists (int[m]) are read on the device: m is their length, offsets outside [0, m] are clamped,
+ * a group that runs backwards has no rows (and where groups overlap, some of their rows may be left out), a row number outside x ([0, x_total)) or y ([0, y_total)) is skipped.  A row of x may be listed any number of times, a row of y
  * once (twice: either result stands, channel by channel).  Rows of y that are not listed are left as they are. */
 int pb_linear_grouped(int device, void *stream, int type, const void *x, uint64_t x_total, uint64_t ldx, const float *x_scale, const void *w, uint64_t ldw,
                       const float *w_scale, const float *bias, const int *offsets, uint32_t groups, const int *x_rows, const int *y_rows, int act,

@@ -1,6 +1,7 @@
 // pb_linear.hip -- C entry points of the linear layers on device buffers (kernels: pb_linear_kernels.h).
 //
-// Each call checks its arguments on the host, queues ONE kernel on the caller's stream and returns.  Nothing is allocated, no
+// Each call checks its arguments on the host, queues one kernel on the caller's stream (quantize_rows one for each 8 or 33 million
+// rows, the heads' product one for as many channels as a launch takes) and returns.  Nothing is allocated, no
 // state outlives a call: calls on any number of streams and from any number of threads are independent, and a captured graph
 // holds nothing that another one shares.
 #include <algorithm>
@@ -69,10 +70,12 @@ bool fits(uint64_t rows, uint64_t ld) { return rows <= 1 || ld <= (1ull << 50) /
 //   wide 256      128: 55    256: 60    512: 123                               52                  62
 // A tile that holds next to no rows costs less (`thin`: its loads of x are of one row); f32 runs at the f32 matrix rate, a sixteenth of
 // the others', and larger tiles gain less there; a longer program starts later when it is not in the instruction caches.  The figures
-// below start from these and are fitted to the times of all forms on 1410 products, dense and grouped, of all types and alignments, 1
-// to 16384 rows, 32 to 8192 channels and values, launched back to back and after other work: the form with the least such cost, which
-// is taken, ran 2.3 and 1.2 % longer than the best one there in the geometric mean.  Sums of 8-bit products are the same by
-// every form.
+// below start from these and are fitted, all together, to the times of all forms on 1410 products, dense and grouped, of all types and
+// alignments, 1 to 16384 rows, 32 to 8192 channels and values, launched back to back and after other work: the form with the least such
+// cost, which is taken, ran 2.3 and 1.2 % longer than the best one there in the geometric mean.  The sum is what was fitted; a single figure
+// need not be that form's time (16 x 16 is costed less on 4 bytes than on 16, tiles of 64 and 128 more on 4 than off them), and beyond
+// those sizes the rule is only a guess between forms that all give the answer.  Sums of 8-bit products are the same by every form; sums
+// of floats are added in an order that goes with the form.
 enum Form { FEW11, FEW21, FEW22, TILE64, TILE128, WIDE128, WIDE256, FORMS };
 struct FormCost {
     int bm, bn, threads, slots;  // tile, workgroup, workgroups per round

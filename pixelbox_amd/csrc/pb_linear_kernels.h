@@ -66,9 +66,10 @@ __device__ __forceinline__ void mma32(typename Acc<T>::q16 &c, const u32x4 &a, c
 
 // ---- loads and stores of any alignment ---------------------------------------------------------------------------------------------------
 // global_load / store_dwordx4 take any address; what that costs depends on the bound.  Tiles load a byte once for many products: on
-// 4 bytes or less they lose what the way through registers costs (4096^3 i8 by 128 x 128: 83 us aligned, 94 on 4 bytes, 125 odd).  The few forms live on loads, which go at full rate on 4 bytes and at a third off them (41 x 217 x 3903 f16: 26.6 us, with
-// 3904 values 10.1): there (DW false) the aligned words around the 16 bytes are read -- only such as hold at least one of them -- and
-// shifted into place (13.0 us; in tiles that costs more than it saves: 777 x 1003 x 1289 i8 12.6 us, plain 11.2).
+// 4 bytes or less they lose what the way through registers costs (4096^3 i8 66 us aligned, 100 on 4 bytes, 134 odd).  The few forms live on
+// loads, which go at full rate on 4 bytes and at a third off them (41 x 217 x 3903 f16: 26.6 us, with 3904 values 10.1): there (DW false)
+// the aligned words around the 16 bytes are read -- only such as hold at least one of them -- and shifted into place (12.9 us; in
+// tiles that costs more than it saves: 777 x 1003 x 1289 i8 with the operands in the caches 12.6 us, plain 11.2).
 template <bool DW>
 __device__ __forceinline__ u32x4 load16(const uint8_t *p) {
     u32x4 v;
@@ -372,8 +373,8 @@ __device__ __forceinline__ void store_tile(const LinearArgs &a, const Chan<T, 8>
 
 // What the tile kernels share: K goes in steps of 128 bytes through NST LDS stages.  A row sits in LDS at a pitch of 128 bytes with its
 // eight 16-byte pieces permuted, so that the fragment reads -- 16 bytes from each of 32 (or of 16 x 4) places -- are free of bank
-// conflicts: with 32-row fragments piece c at c ^ (row / 2 & 7): 249 bytes a clock and CU, against 121 with c ^ (row & 7) and 32
-// unpermuted; with 16-row fragments c ^ (row & 7): 242 (LDS reads alone, 256 workgroups of eight waves).  The permutation is done by
+// conflicts: with 32-row fragments piece c at c ^ (row / 2 & 7): 242 bytes a clock and CU, against 123 with c ^ (row & 7) and 32
+// unpermuted; with 16-row fragments c ^ (row & 7): 232, unpermuted 63 (LDS reads alone, 256 workgroups of eight waves).  The permutation is done by
 // the lanes' GLOBAL addresses, so a wave's eight rows of 128 bytes are still whole lines.  DMA: the
 // loads go straight into LDS (16-byte aligned rows); otherwise through registers, which takes any alignment.  The last, partial step always goes through registers.
 template <int T, int BM, int BN, int NTHR, int NST, bool ROWS16>
@@ -456,8 +457,9 @@ struct Loader {
 // ---- k_linear_tile: small tiles -- 64 x 64 or 128 x 128, waves of 32 x 32 or 64 x 32 ---------------------------------------------------------
 // For products with few tiles, where a step is short: a wave has one or two 32 x 32 matrix instructions to a 32-byte piece, and would
 // wait out an LDS read for each piece, so it reads a step's four pieces at once behind the step's one barrier; four LDS stages give
-// the loads three steps to arrive.  777 x 1003 x 1289 i8 13.6 us, 1024 x 1024 x 1008 7.6.  (4 pieces one after the other: 64 x 4096 x 4096 13.3 us instead of 12.8; two stages: weights out of
-// HBM, 128 x 8192 x 8192, 33.7 us instead of 22.0.)
+// the loads three steps to arrive.  777 x 1003 x 1289 i8 12.5 us (rows of 1296 bytes 9.2), 1024 x 1024 x 1008 7.4.  (By these tiles with 4
+// pieces one after the other 64 x 4096 x 4096 13.3 us instead of 12.8; two stages: weights out of HBM, 128 x 8192 x 8192, 33.7 us instead
+// of 22.0.)
 template <int T, int BM, int BN, int WM, int WN, int NST, bool DMA>
 __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(const LinearArgs a) {
     constexpr int NWM = BM / WM, NWN = BN / WN, NTHR = 64 * NWM * NWN, MT = WM / 32, NT = WN / 32;
@@ -550,8 +552,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_tile(cons
 
 // ---- k_linear_wide: large tiles -- 256 x 256 with waves of 128 x 64, 128 x 128 with waves of 64 x 64 -------------------------------------------
 // For products that fill the chip with such tiles.  16 x 16 matrix instructions: they read and write their sums half as often per
-// multiplication as the 32 x 32 ones, and what limits these products is power (8192^3, clocks fall to 1.75 GHz on random data, the same
-// kernel runs a third faster on zeros): i8 423 us instead of 475, f16 794 instead of 892, bf16 745 instead of 846.
+// multiplication as the 32 x 32 ones, and run faster (bare, without loads: i8 4.09 against 3.38 P/s).  On the same data 8192^3 took i8 423 us
+// instead of 475, f16 794 instead of 892, bf16 745 instead of 846; on evenly spread codes 439, on normally
+// distributed values 825 and 792.  The matrix units
+// are busy 59 % of the cycles (i8; f16 over 32 experts 42 %) at 2.0 GHz (the bare loop: all of them at 1.95); on zeros i8 takes 393 us
+// and f16 662.
 // A step is 2 MT slots, one 16-row fragment of x each (MT pieces of the first 64 bytes, then of the second) against the wave's NT
 // channel fragments.  Fragments of x are read PF slots ahead into a ring of PF + 1, the channels' a half step ahead.  The one
 // barrier of a step stands PF slots before its end, where all that is left of the step is in registers: behind it the step's stage is
@@ -661,11 +666,11 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN)) void k_linear_wide(cons
 }
 
 // ---- k_linear_few: 16 MT rows x 16 NT channels per workgroup, K split over its NW waves ----------------------------------------------------
-// For few rows (or little work): the weights are read once, straight into registers, 256 bytes of a row per wave and turn; the
-// waves' partial sums meet in LDS and are added in wave order.  Bound by the weights out of HBM: 32 rows over 64 groups, 2048 x 2048 bf16
-// (210 MB of 25 groups in use) 41 us, the 5.1 TB/s of a large copy; with weights in the caches by the way from a load
-// to the last sum (16 x 4096 x 4096 i8 7.2 us, 1 x 256 x 1280 4.3 of which 3.3 are any launch's).  Loads a turn ahead would cost
-// registers and with them waves: 40 us instead of 32 (evenly filled groups).
+// For few rows (or little work): the weights are read once, straight into registers, 64 U bytes of a row per wave and turn; the
+// waves' partial sums meet in LDS and are added in wave order, so that a sum's order goes with k and U alone.  Bound by the weights out of
+// HBM: 32 rows over 64 groups, 2048 x 2048 bf16 (210 MB of 25 groups in use) 42 us, 5.0 TB/s (a plain read 5.76, a copy 5.48); with weights in the
+// caches by the way from a load to the last sum (16 x 4096 x 4096 i8 6.4 us, 1 x 256 x 1280 3.1 of which 1.5 are any launch's).  Loads a
+// turn ahead would cost registers and with them waves: 40 us instead of 32 (evenly filled groups).
 template <int T, int MT, int NT, int NW, int U, bool DW>
 __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
     typedef typename Acc<T>::e E;
@@ -775,7 +780,7 @@ __global__ __launch_bounds__(64 * NW) void k_linear_few(const LinearArgs a) {
 // value, and exactly: x * (1 / scale) + 1.5 * 2^23, one fused multiply-add, is the whole number in the low bits (1 / scale is off by
 // half a unit in the last place, the quotient by less than 7.7e-6).  Only where it lies within 1e-5 of a half -- one value in 50 000 -- the
 // remainder x - r * scale decides, which a fused multiply-add gives exactly near scale / 2.  Bound by HBM: 8192 x 1280 f32 (52 MB) 10.0
-// us, the rate of a large copy; 8192 x 8192 bf16 41.5.  A row with an infinity or a NaN gets
+// us, 5.2 TB/s (a copy 5.5); 8192 x 8192 bf16 41.2.  A row with an infinity or a NaN gets
 // scale = NaN and codes 0, so that what is computed from it shows.
 constexpr float MAGIC = 12582912.0f;  // 1.5 * 2^23
 __device__ __forceinline__ uint32_t code_exact(float x, float inv, float scale, float half) {
