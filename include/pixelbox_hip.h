@@ -285,11 +285,11 @@ int pb_embed_features_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, f
  * quantiser of efficientnet.rs:39, all on the embedder's stream (contract as pb_embed_batch_device).  All pointers are DEVICE memory.
  * type: PB_TYPE_F32 (d_w: f32[heads][d][1280]) or PB_TYPE_I8 (int8, with d_w_scale f32[heads][d]: pb_quantize_rows over the weights'
  * rows); d_bias: f32[heads][d] or NULL; d_head: int[n].  d_out_u8: uint8[n][d], d_out_f32: f32[n][d], either may be NULL.  Images
- * whose head is outside [0, heads) are left as they are in both; the outputs overlap neither each other nor
- * d_w, d_w_scale, d_bias or d_head; a call that is refused has queued nothing.  An image's hash does
- * not depend on its batch, nor on the other heads.  The f32 product is summed in plain f32 (the embedder's own Linear
- * sums bf16 pieces): with the blob's own weights as the only head the values agree with pb_embed_batch to the embedding's tolerance,
- * not bit for bit.  An i8 head is off by the codes' rounding: half a code of 254 per feature and weight. */
+ * whose head is outside [0, heads) are left as they are in both; the outputs overlap neither each other nor d_w, d_w_scale, d_bias or
+ * d_head; a call that is refused has queued nothing.  An image's hash does not depend on its batch, nor on the other heads.  The f32
+ * product is summed in plain f32 (the embedder's own Linear sums bf16 pieces): with the blob's own weights as the only head the values
+ * agree with pb_embed_batch to the embedding's tolerance, not bit for bit.  An i8 head is off by the codes' rounding: half a code of
+ * 254 per feature and weight. */
 int pb_embed_heads_device(pb_embedder *e, const uint8_t *d_rgb, uint32_t n, int type, const void *d_w, const float *d_w_scale, const float *d_bias,
                           uint32_t heads, uint32_t d, const int *d_head, uint8_t *d_out_u8, float *d_out_f32);
 
